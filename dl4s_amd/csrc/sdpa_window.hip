@@ -1,0 +1,324 @@
+// Attention with a sliding window and visible first keys for gfx950: forward, gradients, one decoding step over a cache.
+//
+// Query i of batch element b stands at position p = q_offset + i and sees the keys
+//   V(i) = { j : j <= p,  j > p - window or j < sinks,  j < lengths[b] }
+//   s_ij = (q_i * rT) . k_j,   w_ij = exp(s_ij) / sum over V(i) of exp(s_ij'),   out_i = sum over V(i) of w_ij v_j
+// and a row that sees no key has weights and output zero.  H / Hkv consecutive query heads share a key head.  Gradients:
+//   dv_j = sum_i w_ij dout_i,  dS_ij = w_ij (dout_i . v_j - dout_i . out_i),  dq_i = rT sum_j dS_ij k_j,
+//   dk_j = rT sum_i dS_ij q_i  (dk, dv summed over the query heads of the group)
+#include "common.h"
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int MAXD = 256;
+
+struct WindowArgs {
+    int window, sinks;      // clamped to [1, 2^30] and [0, Lk]
+    long long q_offset;
+    const int *lengths;
+    int last_key;           // decode: the query of batch element b stands at position lengths[b] - 1 (or Lk - 1)
+};
+
+// The keys a query sees, as two ranges [0, first) and [lo, hi) with first <= lo.
+struct Range {
+    int first, lo, hi;
+};
+__device__ __forceinline__ Range visible_keys(const WindowArgs &w, const int b, const int i, const int Lk) {
+    int len = w.lengths ? w.lengths[b] : Lk;
+    len = len < 0 ? 0 : (len > Lk ? Lk : len);
+    const long long p = w.last_key ? (long long)len - 1 : w.q_offset + i;
+    Range r;
+    const long long lo = p - w.window + 1;
+    r.hi = (int)(p + 1 < len ? p + 1 : len);
+    r.lo = lo < 0 ? 0 : (int)(lo > r.hi ? r.hi : lo);
+    r.first = w.sinks < r.lo ? w.sinks : r.lo;
+    return r;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+struct Layout {             // element strides of [B, heads, L, d] tensors in either layout
+    long long b, h, l;
+};
+
+// One wavefront per query row, 64 keys at a time: a lane forms the score of one key, then a lane owns up to four output
+// columns.  Any head dim up to 256, any alignment.
+__global__ __launch_bounds__(256) void sdpa_window_rows_f32(const float *__restrict__ q, const float *__restrict__ k,
+                                                             const float *__restrict__ v, float *__restrict__ out,
+                                                             float *__restrict__ stats, int H, int group, int Lq, int Lk, int d,
+                                                             float rT, WindowArgs w, Layout lq, Layout lk, long long rows) {
+    __shared__ float qs[4][MAXD], ps[4][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * 4 + wave;
+    if (row >= rows) return;
+    const int i = (int)(row % Lq);
+    const long long bh = row / Lq;
+    const int h = (int)(bh % H), b = (int)(bh / H);
+    const float *qp = q + b * lq.b + h * lq.h + i * lq.l;
+    const float *kp = k + b * lk.b + (h / group) * lk.h, *vp = v + b * lk.b + (h / group) * lk.h;
+    for (int c = lane; c < d; c += 64) qs[wave][c] = qp[c] * rT;
+    const Range r = visible_keys(w, b, i, Lk);
+    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int part = 0; part < 2; ++part) {
+        const int end = part ? r.hi : r.first;
+        for (int j0 = part ? r.lo : 0; j0 < end; j0 += 64) {
+            const int n = min(64, end - j0);
+            float s = -INFINITY;
+            if (lane < n) {
+                const float *kr = kp + (long long)(j0 + lane) * lk.l;
+                s = 0.f;
+                for (int c = 0; c < d; ++c) s += qs[wave][c] * kr[c];
+                s *= LOG2E;
+            }
+            const float m_new = fmaxf(m, wave_max(s));
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = __builtin_amdgcn_exp2f(m - m_use), p = lane < n ? __builtin_amdgcn_exp2f(s - m_use) : 0.f;
+            m = m_new;
+            l = l * alpha + dl4s::wave_sum(p);
+            ps[wave][lane] = p;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int c = lane + 64 * t;
+                if (c >= d) break;
+                float a = acc[t] * alpha;
+                for (int x = 0; x < n; ++x) a += ps[wave][x] * vp[(long long)(j0 + x) * lk.l + c];
+                acc[t] = a;
+            }
+        }
+    }
+    const float inv = r.first + (r.hi - r.lo) > 0 ? 1.0f / l : 0.f;
+    float *op = out + b * lq.b + h * lq.h + i * lq.l;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        if (lane + 64 * t < d) op[lane + 64 * t] = acc[t] * inv;
+    if (stats && lane == 0) {
+        stats[2 * row] = m == -INFINITY ? 0.f : m;
+        stats[2 * row + 1] = inv;
+    }
+}
+
+// delta_i = dout_i . out_i, one wavefront per row
+__global__ __launch_bounds__(256) void window_delta_f32(const float *__restrict__ dout, const float *__restrict__ out,
+                                                         float *__restrict__ delta, int H, int Lq, int d, Layout lq, long long rows) {
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63;
+    const long long bh = row / Lq, at = (bh / H) * lq.b + (bh % H) * lq.h + (row % Lq) * lq.l;
+    float s = 0.f;
+    for (int c = lane; c < d; c += 64) s += dout[at + c] * out[at + c];
+    s = dl4s::wave_sum(s);
+    if (lane == 0) delta[row] = s;
+}
+
+// dq: one wavefront per query row, the walk of the forward kernel
+__global__ __launch_bounds__(256) void sdpa_window_dq_rows_f32(const float *__restrict__ q, const float *__restrict__ k,
+                                                                const float *__restrict__ v, const float *__restrict__ dout,
+                                                                const float *__restrict__ stats, const float *__restrict__ delta,
+                                                                float *__restrict__ dq, int H, int group, int Lq, int Lk, int d,
+                                                                float rT, WindowArgs w, Layout lq, Layout lk, long long rows) {
+    __shared__ float qs[4][MAXD], gs[4][MAXD], ps[4][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * 4 + wave;
+    if (row >= rows) return;
+    const int i = (int)(row % Lq);
+    const long long bh = row / Lq;
+    const int h = (int)(bh % H), b = (int)(bh / H);
+    const long long at = b * lq.b + h * lq.h + i * lq.l;
+    const float *kp = k + b * lk.b + (h / group) * lk.h, *vp = v + b * lk.b + (h / group) * lk.h;
+    for (int c = lane; c < d; c += 64) {
+        qs[wave][c] = q[at + c] * rT;
+        gs[wave][c] = dout[at + c];
+    }
+    const Range r = visible_keys(w, b, i, Lk);
+    const float m = stats[2 * row], inv = stats[2 * row + 1], del = delta[row];
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int part = 0; part < 2; ++part) {
+        const int end = part ? r.hi : r.first;
+        for (int j0 = part ? r.lo : 0; j0 < end; j0 += 64) {
+            const int n = min(64, end - j0);
+            float ds = 0.f;
+            if (lane < n) {
+                const float *kr = kp + (long long)(j0 + lane) * lk.l, *vr = vp + (long long)(j0 + lane) * lk.l;
+                float s = 0.f, g = 0.f;
+                for (int c = 0; c < d; ++c) { s += qs[wave][c] * kr[c]; g += gs[wave][c] * vr[c]; }
+                ds = __builtin_amdgcn_exp2f(s * LOG2E - m) * inv * (g - del);
+            }
+            ps[wave][lane] = ds;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int c = lane + 64 * t;
+                if (c >= d) break;
+                for (int x = 0; x < n; ++x) acc[t] += ps[wave][x] * kp[(long long)(j0 + x) * lk.l + c];
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        if (lane + 64 * t < d) dq[at + lane + 64 * t] = acc[t] * rT;
+}
+
+// dk, dv: one wavefront per key row, over the queries of the group's heads that can see it, 64 at a time
+__global__ __launch_bounds__(256) void sdpa_window_dkv_rows_f32(const float *__restrict__ q, const float *__restrict__ k,
+                                                                 const float *__restrict__ v, const float *__restrict__ dout,
+                                                                 const float *__restrict__ stats, const float *__restrict__ delta,
+                                                                 float *__restrict__ dk, float *__restrict__ dv, int H, int Hkv,
+                                                                 int Lq, int Lk, int d, float rT, WindowArgs w, Layout lq, Layout lk,
+                                                                 long long rows) {
+    __shared__ float ks[4][MAXD], vs[4][MAXD], ps[4][64], ss[4][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * 4 + wave;
+    if (row >= rows) return;
+    const int j = (int)(row % Lk), group = H / Hkv;
+    const long long bh = row / Lk;
+    const int hk = (int)(bh % Hkv), b = (int)(bh / Hkv);
+    const long long at = b * lk.b + hk * lk.h + j * lk.l;
+    for (int c = lane; c < d; c += 64) {
+        ks[wave][c] = k[at + c];
+        vs[wave][c] = v[at + c];
+    }
+    int len = w.lengths ? w.lengths[b] : Lk;
+    len = len > Lk ? Lk : len;
+    // positions that see key j: from j on, to the window's end unless the key is one of the first
+    long long i0 = (long long)j - w.q_offset, i1 = j < w.sinks ? Lq : (long long)j + w.window - w.q_offset;
+    if (i0 < 0) i0 = 0;
+    if (i1 > Lq) i1 = Lq;
+    if (j >= len) i1 = i0;
+    float ak[4] = {0.f, 0.f, 0.f, 0.f}, av[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int h = hk * group; h < (hk + 1) * group; ++h) {
+        const long long base = b * lq.b + h * lq.h, srow = ((long long)b * H + h) * Lq;
+        for (int q0 = (int)i0; q0 < i1; q0 += 64) {
+            const int n = (int)min(64ll, i1 - q0);
+            float p = 0.f, ds = 0.f;
+            if (lane < n) {
+                const float *qr = q + base + (long long)(q0 + lane) * lq.l, *gr = dout + base + (long long)(q0 + lane) * lq.l;
+                float s = 0.f, g = 0.f;
+                for (int c = 0; c < d; ++c) { s += qr[c] * rT * ks[wave][c]; g += gr[c] * vs[wave][c]; }
+                const long long sr = srow + q0 + lane;
+                p = __builtin_amdgcn_exp2f(s * LOG2E - stats[2 * sr]) * stats[2 * sr + 1];
+                ds = p * (g - delta[sr]);
+            }
+            ps[wave][lane] = p;
+            ss[wave][lane] = ds;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int c = lane + 64 * t;
+                if (c >= d) break;
+                for (int x = 0; x < n; ++x) {
+                    const long long a = base + (long long)(q0 + x) * lq.l + c;
+                    av[t] += ps[wave][x] * dout[a];
+                    ak[t] += ss[wave][x] * q[a];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int c = lane + 64 * t;
+        if (c < d) { dk[at + c] = ak[t] * rT; dv[at + c] = av[t]; }
+    }
+}
+
+inline Layout layout(bool token_major, int64_t heads, int64_t L, int64_t d) {
+    return token_major ? Layout{L * heads * d, d, heads * d} : Layout{heads * L * d, L * d, d};
+}
+inline dim3 row_grid(long long rows) { return dim3((unsigned)((rows + 3) / 4)); }
+
+// What the three entry points check alike.  Returns a status; *w is filled in.
+int window_checks(const char *what, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, const dl4s_window_desc *desc,
+                  uint32_t flags, WindowArgs *w) {
+    DL4S_REQUIRE(B >= 0 && H >= 0 && Hkv >= 0 && Lq >= 0 && Lk >= 0, DL4S_HIP_EINVALID_ARG, "%s: negative extent", what);
+    DL4S_REQUIRE(desc, DL4S_HIP_EINVALID_ARG, "%s: NULL window descriptor", what);
+    DL4S_REQUIRE(desc->window >= 1 && desc->sinks >= 0 && desc->q_offset >= 0, DL4S_HIP_EINVALID_ARG,
+                 "%s: window %lld must be at least 1, sinks %lld and q_offset %lld at least 0", what, (long long)desc->window,
+                 (long long)desc->sinks, (long long)desc->q_offset);
+    DL4S_REQUIRE(!(flags & ~DL4S_SDPA_TOKEN_MAJOR), DL4S_HIP_EINVALID_ARG, "%s: flags %#x (only DL4S_SDPA_TOKEN_MAJOR is known here)", what, flags);
+    DL4S_REQUIRE(H == 0 || (Hkv > 0 && H % Hkv == 0), DL4S_HIP_ESHAPE, "%s: %lld query heads do not share %lld key heads evenly", what,
+                 (long long)H, (long long)Hkv);
+    DL4S_REQUIRE(d >= 1 && d <= MAXD, DL4S_HIP_EUNSUPPORTED, "%s: head dim %lld (1 to %d are implemented)", what, (long long)d, MAXD);
+    const int64_t big = int64_t(1) << 30;
+    DL4S_REQUIRE(Lq < big && Lk < big && B < big && H < big && B * H < big && desc->q_offset < big, DL4S_HIP_EUNSUPPORTED,
+                 "%s: an extent or the offset above 2^30", what);
+    DL4S_REQUIRE(B * H * Lq < big * 4 && B * Hkv * Lk < big * 4, DL4S_HIP_EUNSUPPORTED, "%s: more than 2^32 rows", what);
+    w->window = (int)(desc->window < big ? desc->window : big);
+    w->sinks = (int)(desc->sinks < Lk ? desc->sinks : Lk);
+    w->q_offset = desc->q_offset;
+    w->lengths = desc->lengths;
+    w->last_key = 0;
+    return DL4S_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats,
+                                 int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float inv_temperature,
+                                 const dl4s_window_desc *window, uint32_t flags) {
+    DL4S_CHECK_CTX(ctx);
+    WindowArgs w;
+    const int rc = window_checks("sdpa_window_fwd", B, H, Hkv, Lq, Lk, d, window, flags, &w);
+    if (rc) return rc;
+    const long long rows = (long long)B * H * Lq;
+    if (rows == 0) return DL4S_HIP_OK;
+    DL4S_REQUIRE(q && out && (Lk == 0 || (k && v)), DL4S_HIP_EINVALID_ARG, "sdpa_window_fwd: NULL tensor pointer");
+    const bool tm = flags & DL4S_SDPA_TOKEN_MAJOR;
+    hipLaunchKernelGGL(sdpa_window_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, k, v, out, stats, (int)H, (int)(H / Hkv),
+                       (int)Lq, (int)Lk, (int)d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d), rows);
+    return dl4s::launch_status("sdpa_window_rows_f32");
+}
+
+int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
+                                 const float *stats, const float *dout, float *dq, float *dk, float *dv, int64_t B, int64_t H,
+                                 int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float inv_temperature, const dl4s_window_desc *window,
+                                 uint32_t flags) {
+    DL4S_CHECK_CTX(ctx);
+    WindowArgs w;
+    int rc = window_checks("sdpa_window_bwd", B, H, Hkv, Lq, Lk, d, window, flags, &w);
+    if (rc) return rc;
+    const long long rows = (long long)B * H * Lq, krows = (long long)B * Hkv * Lk;
+    if (rows == 0 && krows == 0) return DL4S_HIP_OK;
+    DL4S_REQUIRE((rows == 0 || (q && out && stats && dout && dq)) && (krows == 0 || (k && v && dk && dv)), DL4S_HIP_EINVALID_ARG,
+                 "sdpa_window_bwd: NULL tensor pointer");
+    const bool tm = flags & DL4S_SDPA_TOKEN_MAJOR;
+    const Layout lq = layout(tm, H, Lq, d), lk = layout(tm, Hkv, Lk, d);
+    std::unique_lock<std::mutex> scratch_lock(ctx->scratch_mu);
+    rc = dl4s::ensure_scratch(ctx, (size_t)rows * sizeof(float));
+    if (rc) return rc;
+    float *delta = reinterpret_cast<float *>(ctx->scratch);
+    if (rows) {
+        hipLaunchKernelGGL(window_delta_f32, row_grid(rows), dim3(256), 0, ctx->stream, dout, out, delta, (int)H, (int)Lq, (int)d, lq, rows);
+        hipLaunchKernelGGL(sdpa_window_dq_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, k, v, dout, stats, delta, dq, (int)H,
+                           (int)(H / Hkv), (int)Lq, (int)Lk, (int)d, inv_temperature, w, lq, lk, rows);
+        rc = dl4s::launch_status("sdpa_window_dq_rows_f32");
+        if (rc) return rc;
+    }
+    if (krows)
+        hipLaunchKernelGGL(sdpa_window_dkv_rows_f32, row_grid(krows), dim3(256), 0, ctx->stream, q, k, v, dout, stats, delta, dk, dv,
+                           (int)H, (int)Hkv, (int)Lq, (int)Lk, (int)d, inv_temperature, w, lq, lk, krows);
+    return dl4s::launch_status("sdpa_window_dkv_rows_f32");
+}
+
+int dl4s_hip_sdpa_window_decode_f32(dl4s_hip_ctx *ctx, const float *q, const float *kcache, const float *vcache, float *out, int64_t B,
+                                    int64_t H, int64_t Hkv, int64_t T, int64_t Tcap, int64_t d, float inv_temperature, int64_t window,
+                                    int64_t sinks, const int32_t *lengths) {
+    DL4S_CHECK_CTX(ctx);
+    const dl4s_window_desc desc = {window, sinks, 0, lengths};
+    WindowArgs w;
+    const int rc = window_checks("sdpa_window_decode", B, H, Hkv, 1, Tcap, d, &desc, 0, &w);
+    if (rc) return rc;
+    const long long rows = (long long)B * H;
+    if (rows == 0) return DL4S_HIP_OK;
+    DL4S_REQUIRE(q && kcache && vcache && out, DL4S_HIP_EINVALID_ARG, "sdpa_window_decode: NULL tensor pointer");
+    DL4S_REQUIRE(T >= 1 && T <= Tcap, DL4S_HIP_ESHAPE, "sdpa_window_decode: T=%lld must be in [1, Tcap=%lld]", (long long)T, (long long)Tcap);
+    w.last_key = 1;
+    hipLaunchKernelGGL(sdpa_window_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, kcache, vcache, out, (float *)nullptr, (int)H,
+                       (int)(H / Hkv), 1, (int)T, (int)d, inv_temperature, w, layout(false, H, 1, d), layout(false, Hkv, Tcap, d), rows);
+    return dl4s::launch_status("sdpa_window_rows_f32");
+}
+
+}  // extern "C"

@@ -17,6 +17,8 @@ SDPA_TOKEN_MAJOR = 2
 SDPA_NO_KEY_SPLIT = 4
 ACT_NONE, ACT_GELU = 0, 1
 OP_ADD, OP_SUB, OP_MUL, OP_DIV = range(4)
+ROTARY_INTERLEAVED, ROTARY_INVERSE, ROTARY_TOKEN_MAJOR = 1, 2, 4
+ROTARY_UNSCALED, ROTARY_SCALE_POSITIONS, ROTARY_SCALE_BASE, ROTARY_SCALE_BY_PARTS = range(4)
 
 _vp = C.c_void_p
 _i64 = C.c_int64
@@ -24,6 +26,10 @@ _i64 = C.c_int64
 
 class MaskDesc(C.Structure):
     _fields_ = [("kind", C.c_int32), ("dense", _vp), ("shape", _i64 * 4), ("lengths", _vp), ("classes", _vp)]
+
+
+class WindowDesc(C.Structure):
+    _fields_ = [("window", _i64), ("sinks", _i64), ("q_offset", _i64), ("lengths", _vp)]
 
 
 class Dl4sHipError(RuntimeError):
@@ -80,6 +86,14 @@ class DeviceBuffer:
 
 def _shape_arr(shape):
     return (_i64 * max(1, len(shape)))(*shape)
+
+
+def rotary_frequencies(rot_dim, base=10000.0, scaling=ROTARY_UNSCALED, factor=1.0, low=1.0, high=32.0, original_length=0):
+    """Turns per position of each pair of columns, float64 [rot_dim / 2] in host memory (dl4s_hip_rotary_frequencies)."""
+    out = np.empty(max(int(rot_dim), 0) // 2, np.float64)
+    _check(load().dl4s_hip_rotary_frequencies(_i64(rot_dim), C.c_double(base), int(scaling), C.c_double(factor), C.c_double(low),
+                                              C.c_double(high), _i64(original_length), out.ctypes.data_as(_vp)))
+    return out
 
 
 def graph_supported():
@@ -258,6 +272,41 @@ class Context:
                                                          _vp(_ptr(k_new)), _vp(_ptr(v_new)), _vp(_ptr(out)), _i64(B), _i64(H),
                                                          _vp(_ptr(pos_dev)), _i64(Tcap), _i64(d), C.c_float(inv_temperature)))
 
+    # ---- attention with a sliding window, rotary positions (lengths, positions, counts: device int32; turns: device float64)
+    def window_desc(self, window, sinks=0, q_offset=0, lengths=None):
+        return WindowDesc(window, sinks, q_offset, _opt(lengths))
+
+    def sdpa_window_fwd(self, q, k, v, out, stats, B, H, Hkv, Lq, Lk, d, inv_temperature, window, flags=0):
+        """window: a window_desc; stats: [B,H,Lq,2] for sdpa_window_bwd, or None."""
+        _check(self.lib.dl4s_hip_sdpa_window_fwd_f32(self.handle, _vp(_ptr(q)), _vp(_ptr(k)), _vp(_ptr(v)), _vp(_ptr(out)),
+                                                     _vp(_opt(stats)), _i64(B), _i64(H), _i64(Hkv), _i64(Lq), _i64(Lk), _i64(d),
+                                                     C.c_float(inv_temperature), C.byref(window), C.c_uint32(flags)))
+
+    def sdpa_window_bwd(self, q, k, v, out, stats, dout, dq, dk, dv, B, H, Hkv, Lq, Lk, d, inv_temperature, window, flags=0):
+        _check(self.lib.dl4s_hip_sdpa_window_bwd_f32(self.handle, _vp(_ptr(q)), _vp(_ptr(k)), _vp(_ptr(v)), _vp(_ptr(out)),
+                                                     _vp(_ptr(stats)), _vp(_ptr(dout)), _vp(_ptr(dq)), _vp(_ptr(dk)), _vp(_ptr(dv)),
+                                                     _i64(B), _i64(H), _i64(Hkv), _i64(Lq), _i64(Lk), _i64(d),
+                                                     C.c_float(inv_temperature), C.byref(window), C.c_uint32(flags)))
+
+    def sdpa_window_decode(self, q, kcache, vcache, out, B, H, Hkv, T, Tcap, d, inv_temperature, window, sinks=0, lengths=None):
+        _check(self.lib.dl4s_hip_sdpa_window_decode_f32(self.handle, _vp(_ptr(q)), _vp(_ptr(kcache)), _vp(_ptr(vcache)),
+                                                        _vp(_ptr(out)), _i64(B), _i64(H), _i64(Hkv), _i64(T), _i64(Tcap), _i64(d),
+                                                        C.c_float(inv_temperature), _i64(window), _i64(sinks), _vp(_opt(lengths))))
+
+    def rotary(self, q, q_out, k, k_out, B, L, H, Hkv, d, rot_dim, turns, positions=None, position0=0, amplitude=1.0, flags=0):
+        """positions: [B,L], or None for position0 + l."""
+        _check(self.lib.dl4s_hip_rotary_f32(self.handle, _vp(_opt(q)), _vp(_opt(q_out)), _vp(_opt(k)), _vp(_opt(k_out)), _i64(B),
+                                            _i64(L), _i64(H), _i64(Hkv), _i64(d), _i64(rot_dim), _vp(_opt(turns)),
+                                            _vp(_opt(positions)), _i64(position0), C.c_float(amplitude), C.c_uint32(flags)))
+
+    def rotary_append(self, q, k_new, v_new, q_out, kcache, vcache, B, L, H, Hkv, Tcap, d, rot_dim, turns, positions=None, position0=0,
+                      counts=None, amplitude=1.0, flags=0):
+        """positions: [B], or None for position0; counts: rows written of each batch element's L, or None for all."""
+        _check(self.lib.dl4s_hip_rotary_append_f32(self.handle, _vp(_opt(q)), _vp(_opt(k_new)), _vp(_opt(v_new)), _vp(_opt(q_out)),
+                                                   _vp(_opt(kcache)), _vp(_opt(vcache)), _i64(B), _i64(L), _i64(H), _i64(Hkv),
+                                                   _i64(Tcap), _i64(d), _i64(rot_dim), _vp(_opt(turns)), _vp(_opt(positions)),
+                                                   _i64(position0), _vp(_opt(counts)), C.c_float(amplitude), C.c_uint32(flags)))
+
     # ---- engine primitives
     def fill(self, value, result, count):
         _check(self.lib.dl4s_hip_fill_f32(self.handle, C.c_float(value), _vp(_ptr(result)), _i64(count)))
@@ -311,6 +360,20 @@ class Context:
 
     def log_softmax(self, x, rows, n, y):
         _check(self.lib.dl4s_hip_log_softmax_f32(self.handle, _vp(_ptr(x)), _i64(rows), _i64(n), _vp(_ptr(y))))
+
+    def token_logprobs(self, logits, rows, n, row_stride, targets, logprobs, entropy=None, stats=None, inv_temperature=1.0,
+                       ignore_index=-1, top_k=0, top_logprobs=None, top_tokens=None):
+        _check(self.lib.dl4s_hip_token_logprobs_f32(self.handle, _vp(_opt(logits)), _i64(rows), _i64(n), _i64(row_stride),
+                                                    C.c_float(inv_temperature), _vp(_opt(targets)), C.c_int32(ignore_index),
+                                                    _vp(_opt(logprobs)), _vp(_opt(entropy)), _vp(_opt(stats)), _i64(top_k),
+                                                    _vp(_opt(top_logprobs)), _vp(_opt(top_tokens))))
+
+    def token_logprobs_bwd(self, logits, rows, n, row_stride, targets, stats, dlogits, dlogprobs=None, dentropy=None,
+                           inv_temperature=1.0, ignore_index=-1):
+        _check(self.lib.dl4s_hip_token_logprobs_bwd_f32(self.handle, _vp(_opt(logits)), _i64(rows), _i64(n), _i64(row_stride),
+                                                        C.c_float(inv_temperature), _vp(_opt(targets)), C.c_int32(ignore_index),
+                                                        _vp(_opt(stats)), _vp(_opt(dlogprobs)), _vp(_opt(dentropy)),
+                                                        _vp(_opt(dlogits))))
 
     def gemm(self, lhs, lshape, rhs, rshape, result, alpha=1.0, beta=0.0, ta=False, tb=False):
         _check(self.lib.dl4s_hip_gemm_f32(self.handle, _vp(_ptr(lhs)), _i64(lshape[0]), _i64(lshape[1]), _vp(_ptr(rhs)),
@@ -395,3 +458,8 @@ class Context:
 def _ptr(x):
     """DeviceBuffer or raw integer device address."""
     return x.ptr if isinstance(x, DeviceBuffer) else int(x)
+
+
+def _opt(x):
+    """The same, or NULL for None."""
+    return None if x is None else _ptr(x)

@@ -290,6 +290,79 @@ int dl4s_hip_sdpa_decode_step_at_f32(dl4s_hip_ctx *ctx, const float *q, float *k
 int dl4s_hip_argmax_to_f32(dl4s_hip_ctx *ctx, const float *values, int64_t count, int32_t *out_index_dev,
                            int32_t *counter_dev);
 
+/* ------------------------------------------------ attention with a sliding window and visible first keys
+ * No counterpart in the reference, whose masks are full, causal or key lengths.  Query row i of batch element b stands at
+ * position p = q_offset + i and sees key j when  j <= p,  j > p - window or j < sinks,  and j < lengths[b]:
+ *   out = softmax over the visible keys of ((q * inv_temperature) . k^T) . v
+ * A row that sees no key (a length of zero, a window that lies behind the last valid key) has output zero and takes part in
+ * no gradient.  q, out [B,H,Lq,d], k, v [B,Hkv,Lk,d], or [B,L,heads,d] with DL4S_SDPA_TOKEN_MAJOR; row-major fp32 without
+ * gaps.  Hkv divides H, and H / Hkv consecutive query heads read the same key head.  d from 1 to 256, any alignment of the
+ * pointers.  The outputs may not overlap the inputs.  K and V are taken to be finite at keys that are hidden from some
+ * queries and visible to others of the same 32 (a NaN or infinity there reaches those other rows' neighbours too); rows at
+ * or beyond lengths[b] are never used and may hold anything.  An infinite q, k, v or dout gives NaN. */
+typedef struct dl4s_window_desc {
+    int64_t window;         /* >= 1: the query's own position and the window - 1 before it */
+    int64_t sinks;          /* >= 0: the first keys, which stay visible to every later position */
+    int64_t q_offset;       /* >= 0: position of query row 0 (Lk - Lq when the queries are the last rows of the keys) */
+    const int32_t *lengths; /* device int32 [B]: valid keys of each batch element, or NULL */
+} dl4s_window_desc;
+
+/* The forward pass; stats [B,H,Lq,2] (opaque, for the gradient call) may be NULL.  Only DL4S_SDPA_TOKEN_MAJOR is known in flags. */
+int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats,
+                                 int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float inv_temperature,
+                                 const dl4s_window_desc *window, uint32_t flags);
+/* dq, dk, dv for the upstream gradient dout, from the tensors of the forward call with the same extents, window and flags.
+ * dk and dv are summed over the query heads that share a key head.  Deterministic: no atomics, the same bits on every run.
+ * Uses the library's scratch block. */
+int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
+                                 const float *stats, const float *dout, float *dq, float *dk, float *dv, int64_t B, int64_t H,
+                                 int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float inv_temperature, const dl4s_window_desc *window,
+                                 uint32_t flags);
+/* One decoding step: q, out [B,H,1,d] over caches [B,Hkv,Tcap,d] whose first lengths[b] rows are valid (device int32 [B];
+ * NULL: T rows everywhere; values are clamped to [0, T]).  The query stands at the last valid row: it sees the last `window`
+ * rows and the first `sinks`.  A length of zero gives zeros.  T is the largest length there can be, so that the call can be
+ * recorded once and replayed while the lengths grow in device memory. */
+int dl4s_hip_sdpa_window_decode_f32(dl4s_hip_ctx *ctx, const float *q, const float *kcache, const float *vcache, float *out, int64_t B,
+                                    int64_t H, int64_t Hkv, int64_t T, int64_t Tcap, int64_t d, float inv_temperature, int64_t window,
+                                    int64_t sinks, const int32_t *lengths);
+
+/* ------------------------------------------------ rotary positions
+ * No counterpart in the reference, which adds sinusoidal positions to the embeddings (PositionalEncoding.swift:52-69).  The
+ * first rot_dim columns of every query and key head turn in pairs (a, b), pair i by turns[i] full turns per position:
+ *   y_a = amplitude * (x_a cos - x_b sin),  y_b = amplitude * (x_a sin + x_b cos),  angle = 2 pi * turns[i] * position
+ * (a, b) = (i, i + rot_dim / 2), or (2i, 2i + 1) with DL4S_ROTARY_INTERLEAVED; the other columns are copied.  The angle is
+ * reduced in 64 bits, so far positions keep their precision. */
+#define DL4S_ROTARY_INTERLEAVED 1u
+#define DL4S_ROTARY_INVERSE 2u      /* turn back: the transposed map, which is the gradient (amplitude * (-angle)) */
+#define DL4S_ROTARY_TOKEN_MAJOR 4u  /* tensors [B,L,heads,d] instead of [B,heads,L,d] */
+/* Fills out_turns[rot_dim / 2] (HOST memory, host arithmetic only; copy it to the device once): base^(-2i / rot_dim) / (2 pi),
+ * and for contexts longer than the model was trained on, stretched by `factor`:
+ *   SCALE_POSITIONS  every frequency divided by factor
+ *   SCALE_BASE       base * factor^(rot_dim / (rot_dim - 2)) in place of base
+ *   SCALE_BY_PARTS   pairs that make fewer than `low` turns over original_length positions divided by factor, pairs that make
+ *                    more than `high` kept, a linear blend between */
+typedef enum dl4s_rotary_scaling {
+    DL4S_ROTARY_UNSCALED = 0,
+    DL4S_ROTARY_SCALE_POSITIONS = 1,
+    DL4S_ROTARY_SCALE_BASE = 2,
+    DL4S_ROTARY_SCALE_BY_PARTS = 3
+} dl4s_rotary_scaling;
+int dl4s_hip_rotary_frequencies(int64_t rot_dim, double base, int scaling, double factor, double low, double high,
+                                int64_t original_length, double *out_turns);
+/* Queries and keys in one launch (either pair of pointers may be NULL with its head count 0); an output may be its input.
+ * positions: device int32 [B,L], or NULL for position0 + l. */
+int dl4s_hip_rotary_f32(dl4s_hip_ctx *ctx, const float *q, float *q_out, const float *k, float *k_out, int64_t B, int64_t L, int64_t H,
+                        int64_t Hkv, int64_t d, int64_t rot_dim, const double *turns, const int32_t *positions, int64_t position0,
+                        float amplitude, uint32_t flags);
+/* L new rows per batch element: turned queries to q_out, turned keys and the values into the caches [B,Hkv,Tcap,d].  The rows
+ * of batch element b stand at positions[b] + l (device int32 [B], or NULL for position0 + l), which is also their cache row;
+ * only the first counts[b] of them are written when counts (device int32 [B]) is given, and a row outside [0, Tcap) is not
+ * written.  The queries of all L rows are turned.  DL4S_ROTARY_INVERSE is refused. */
+int dl4s_hip_rotary_append_f32(dl4s_hip_ctx *ctx, const float *q, const float *k_new, const float *v_new, float *q_out, float *kcache,
+                               float *vcache, int64_t B, int64_t L, int64_t H, int64_t Hkv, int64_t Tcap, int64_t d, int64_t rot_dim,
+                               const double *turns, const int32_t *positions, int64_t position0, const int32_t *counts, float amplitude,
+                               uint32_t flags);
+
 /* ------------------------------------------------------------------ EngineType subset */
 /* The primitives the layers on the path call (Engine/Engine.swift:143-581); fp32 only.
  * `result` may alias an input wherever the reference allows it (same-shape elementwise ops). */
@@ -409,6 +482,22 @@ int dl4s_hip_embed_positions_f32(dl4s_hip_ctx *ctx, const float *table, int64_t 
                                  float *result);
 /* logSoftmax over the last axis of x [rows, n] (Tensor/Operators/Unary.swift:198-204): (x - max) - log(sum(exp(x - max))). */
 int dl4s_hip_log_softmax_f32(dl4s_hip_ctx *ctx, const float *x, int64_t rows, int64_t n, float *result);
+/* Log probabilities of given tokens.  logits [rows, n] with row_stride >= n floats between rows; z = logits * inv_temperature:
+ *   logprobs[r] = log softmax(z_r)[targets[r]]       0 for a target equal to ignore_index, NaN for one outside [0, n)
+ *   entropy[r]  = -sum p log p                       a blocked token (z = -inf) adds nothing
+ *   top_logprobs, top_tokens [rows, top_k]           the top_k largest z of the row in order, equal ones by the lower token
+ *                                                    (NaN comes last); top_k <= n, up to 64
+ * targets and logprobs come together or are both NULL; entropy and stats may be NULL.  stats [rows,3] is opaque, for the
+ * gradient call.  No counterpart in the reference, which forms all n log probabilities (Tensor/Operators/Unary.swift:198-204). */
+int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t rows, int64_t n, int64_t row_stride,
+                                float inv_temperature, const int32_t *targets, int32_t ignore_index, float *logprobs, float *entropy,
+                                float *stats, int64_t top_k, float *top_logprobs, int32_t *top_tokens);
+/* dlogits [rows, n] (rows row_stride apart; may be logits itself; columns from n on are left as they are) for the upstream
+ * gradients dlogprobs [rows] and dentropy [rows], each of which may be NULL.  An ignored row takes no gradient through its
+ * log probability, a target outside [0, n) gives NaN. */
+int dl4s_hip_token_logprobs_bwd_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t rows, int64_t n, int64_t row_stride,
+                                    float inv_temperature, const int32_t *targets, int32_t ignore_index, const float *stats,
+                                    const float *dlogprobs, const float *dentropy, float *dlogits);
 /* The Dense layer with its neighbours folded into the product's epilogue:
  *   result = act(x . weights + bias) + residual
  * x [rows, in], weights [in, out], bias [out] or NULL, residual [rows, out] or NULL, result [rows, out].
