@@ -6,45 +6,17 @@
 // and a row that sees no key has weights and output zero.  H / Hkv consecutive query heads share a key head.  Gradients:
 //   dv_j = sum_i w_ij dout_i,  dS_ij = w_ij (dout_i . v_j - dout_i . out_i),  dq_i = rT sum_j dS_ij k_j,
 //   dk_j = rT sum_i dS_ij q_i  (dk, dv summed over the query heads of the group)
-#include "common.h"
+#include <initializer_list>
+
+#include "sdpa_window_fwd.h"
 
 namespace {
-
-constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int MAXD = 256;
-
-struct WindowArgs {
-    int window, sinks;      // clamped to [1, 2^30] and [0, Lk]
-    long long q_offset;
-    const int *lengths;
-    int last_key;           // decode: the query of batch element b stands at position lengths[b] - 1 (or Lk - 1)
-};
-
-// The keys a query sees, as two ranges [0, first) and [lo, hi) with first <= lo.
-struct Range {
-    int first, lo, hi;
-};
-__device__ __forceinline__ Range visible_keys(const WindowArgs &w, const int b, const int i, const int Lk) {
-    int len = w.lengths ? w.lengths[b] : Lk;
-    len = len < 0 ? 0 : (len > Lk ? Lk : len);
-    const long long p = w.last_key ? (long long)len - 1 : w.q_offset + i;
-    Range r;
-    const long long lo = p - w.window + 1;
-    r.hi = (int)(p + 1 < len ? p + 1 : len);
-    r.lo = lo < 0 ? 0 : (int)(lo > r.hi ? r.hi : lo);
-    r.first = w.sinks < r.lo ? w.sinks : r.lo;
-    return r;
-}
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
-
-struct Layout {             // element strides of [B, heads, L, d] tensors in either layout
-    long long b, h, l;
-};
 
 // One wavefront per query row, 64 keys at a time: a lane forms the score of one key, then a lane owns up to four output
 // columns.  Any head dim up to 256, any alignment.
@@ -228,6 +200,49 @@ inline Layout layout(bool token_major, int64_t heads, int64_t L, int64_t d) {
 }
 inline dim3 row_grid(long long rows) { return dim3((unsigned)((rows + 3) / 4)); }
 
+inline bool on_16_bytes(std::initializer_list<const void *> ps) {
+    uintptr_t bits = 0;
+    for (const void *p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+    return (bits & 15) == 0;
+}
+
+// Query heads of a group that one workgroup takes together, and the rest of the launch.
+WindowGeometry geometry(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float rT, bool token_major, bool aligned,
+                        const WindowArgs &w) {
+    WindowGeometry g;
+    g.H = (int)H; g.Hkv = (int)Hkv; g.group = (int)(H / Hkv); g.Lq = (int)Lq; g.Lk = (int)Lk; g.d = (int)d;
+    g.hp = g.group % 4 == 0 ? 4 : (g.group % 2 == 0 ? 2 : 1);
+    g.nqb = (int)((Lq + 128 / g.hp - 1) / (128 / g.hp));
+    g.units = (int)(B * Hkv * (g.group / g.hp) * g.nqb);
+    g.per_xcd = (g.units + 7) / 8;
+    g.rT = rT;
+    g.vec = aligned && d % 4 == 0;
+    g.lq = layout(token_major, H, Lq, d);
+    g.lk = layout(token_major, Hkv, Lk, d);
+    g.w = w;
+    return g;
+}
+
+// Kernels with more than 64 KiB of LDS have their limit raised once per device.
+template <typename K>
+int lds_limit(dl4s_hip_ctx *ctx, int kind, K kernel, size_t bytes) {
+    if (bytes > 65536 && dl4s::lds_limit_pending(ctx, dl4s::LDS_WINDOW, kind)) {
+        DL4S_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        dl4s::lds_limit_done(ctx, dl4s::LDS_WINDOW, kind);
+    }
+    return DL4S_HIP_OK;
+}
+
+template <int DT, int BN>
+int launch_fwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, const WindowGeometry &g) {
+    typedef Tile<BN, DT> T;
+    const size_t lds = 2 * 3 * (T::ROWS_PLANE + T::COLS_PLANE);
+    const int rc = lds_limit(ctx, DT / 32 - 1, sdpa_window_fwd_f32<DT, BN>, lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((sdpa_window_fwd_f32<DT, BN>), dim3(8 * g.per_xcd), dim3(256), lds, ctx->stream, q, k, v, out, stats, g);
+    return dl4s::launch_status("sdpa_window_fwd_f32");
+}
+
 // What the three entry points check alike.  Returns a status; *w is filled in.
 int window_checks(const char *what, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, const dl4s_window_desc *desc,
                   uint32_t flags, WindowArgs *w) {
@@ -267,6 +282,13 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     if (rows == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE(q && out && (Lk == 0 || (k && v)), DL4S_HIP_EINVALID_ARG, "sdpa_window_fwd: NULL tensor pointer");
     const bool tm = flags & DL4S_SDPA_TOKEN_MAJOR;
+    if (d <= 128) {
+        const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, on_16_bytes({q, k, v, out}), w);
+        if (d <= 32) return launch_fwd<32, 64>(ctx, q, k, v, out, stats, g);
+        if (d <= 64) return launch_fwd<64, 64>(ctx, q, k, v, out, stats, g);
+        if (d <= 96) return launch_fwd<96, 32>(ctx, q, k, v, out, stats, g);
+        return launch_fwd<128, 32>(ctx, q, k, v, out, stats, g);
+    }
     hipLaunchKernelGGL(sdpa_window_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, k, v, out, stats, (int)H, (int)(H / Hkv),
                        (int)Lq, (int)Lk, (int)d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d), rows);
     return dl4s::launch_status("sdpa_window_rows_f32");
