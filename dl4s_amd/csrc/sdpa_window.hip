@@ -6,9 +6,10 @@
 // and a row that sees no key has weights and output zero.  H / Hkv consecutive query heads share a key head.  Gradients:
 //   dv_j = sum_i w_ij dout_i,  dS_ij = w_ij (dout_i . v_j - dout_i . out_i),  dq_i = rT sum_j dS_ij k_j,
 //   dk_j = rT sum_i dS_ij q_i  (dk, dv summed over the query heads of the group)
+#include <algorithm>
 #include <initializer_list>
 
-#include "sdpa_window_fwd.h"
+#include "sdpa_window_bwd.h"
 
 namespace {
 
@@ -243,6 +244,59 @@ int launch_fwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v
     return dl4s::launch_status("sdpa_window_fwd_f32");
 }
 
+// Deals the key blocks to workgroups.  A block that every later query sees (first keys) gets about as many query tiles per
+// workgroup as a block that only its window's queries see, and all get more workgroups while there are fewer than two per
+// compute unit; at most 2048 workgroups leave partial sums.
+KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B) {
+    KeyBlocks kb;
+    kb.pairs = (int)(B * g.Hkv);
+    kb.blocks = (g.Lk + 127) / 128;
+    kb.sink_blocks = std::min(kb.blocks, (g.w.sinks + 127) / 128);
+    const long long tiles = (g.Lq + 31) / 32, near = std::min<long long>(tiles, (g.w.window + 127ll + 31) / 32 + 1);
+    const long long n[2] = {tiles * g.group, near * g.group}, count[2] = {(long long)kb.pairs * kb.sink_blocks, (long long)kb.pairs * (kb.blocks - kb.sink_blocks)};
+    const long long fill = (2ll * ctx->cu_count + kb.pairs * (long long)kb.blocks - 1) / (kb.pairs * (long long)kb.blocks);
+    long long floats = 0;
+    for (int c = 0; c < 2; ++c) {
+        long long chunks = std::max(fill, c ? 1 : (tiles + near - 1) / near);
+        chunks = std::min(chunks, std::max(1ll, n[c] / 4));
+        chunks = std::min(chunks, std::max(1ll, 2048 / std::max(1ll, count[c])));
+        kb.chunks[c] = (int)chunks;
+        kb.units[c] = (int)(count[c] * chunks);
+        kb.per_xcd[c] = (kb.units[c] + 7) / 8;
+        if (c) kb.class1 = floats;
+        if (chunks > 1) floats += count[c] * chunks * 256 * g.d;
+    }
+    kb.partial = reinterpret_cast<float *>(floats * sizeof(float));      // the caller replaces the size by the address
+    return kb;
+}
+
+template <int DT>
+int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats, const float *dout,
+               float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
+    typedef Tile<32, DT> T;
+    const size_t lds_q = 2 * 3 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 3 * (2 * T::ROWS_PLANE + 2 * T::COLS_PLANE) + 96 * sizeof(float);
+    int rc = lds_limit(ctx, DT / 32 - 1, sdpa_window_dq_f32<DT>, lds_q);
+    if (!rc) rc = lds_limit(ctx, 4 + DT / 32 - 1, sdpa_window_dkv_f32<DT>, lds_k);
+    if (rc) return rc;
+    if (g.units) {
+        hipLaunchKernelGGL((sdpa_window_dq_f32<DT>), dim3(8 * g.per_xcd), dim3(256), lds_q, ctx->stream, q, k, v, out, stats, dout, dq, delta, g);
+        rc = dl4s::launch_status("sdpa_window_dq_f32");
+        if (rc) return rc;
+    }
+    if (kb.pairs && kb.blocks) {
+        hipLaunchKernelGGL((sdpa_window_dkv_f32<DT>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1])), dim3(256), lds_k, ctx->stream, q, k, v, stats,
+                           dout, delta, dk, dv, g, kb);
+        rc = dl4s::launch_status("sdpa_window_dkv_f32");
+        for (int c = 0; c < 2 && !rc; ++c) {
+            const int first = c ? kb.sink_blocks : 0, n = c ? kb.blocks - kb.sink_blocks : kb.sink_blocks;
+            if (kb.chunks[c] == 1 || n == 0) continue;
+            hipLaunchKernelGGL(sdpa_window_join_f32, dim3(g.d, n, kb.pairs), dim3(256), 0, ctx->stream, dk, dv, g, kb, first);
+            rc = dl4s::launch_status("sdpa_window_join_f32");
+        }
+    }
+    return rc;
+}
+
 // What the three entry points check alike.  Returns a status; *w is filled in.
 int window_checks(const char *what, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, const dl4s_window_desc *desc,
                   uint32_t flags, WindowArgs *w) {
@@ -309,7 +363,20 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     const bool tm = flags & DL4S_SDPA_TOKEN_MAJOR;
     const Layout lq = layout(tm, H, Lq, d), lk = layout(tm, Hkv, Lk, d);
     std::unique_lock<std::mutex> scratch_lock(ctx->scratch_mu);
-    rc = dl4s::ensure_scratch(ctx, (size_t)rows * sizeof(float));
+    const size_t delta_bytes = ((size_t)rows * sizeof(float) + 255) / 256 * 256;
+    if (d <= 128 && H > 0) {
+        const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, on_16_bytes({q, k, v, out, dout, dq, dk, dv}), w);
+        KeyBlocks kb = krows ? key_blocks(ctx, g, B) : KeyBlocks{};
+        rc = dl4s::ensure_scratch(ctx, delta_bytes + reinterpret_cast<size_t>(kb.partial));
+        if (rc) return rc;
+        float *delta = reinterpret_cast<float *>(ctx->scratch);
+        kb.partial = delta + delta_bytes / sizeof(float);
+        if (d <= 32) return launch_bwd<32>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+        if (d <= 64) return launch_bwd<64>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+        if (d <= 96) return launch_bwd<96>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+        return launch_bwd<128>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+    }
+    rc = dl4s::ensure_scratch(ctx, delta_bytes);
     if (rc) return rc;
     float *delta = reinterpret_cast<float *>(ctx->scratch);
     if (rows) {
