@@ -3,7 +3,13 @@
 //   y_a = amplitude (x_a cos - x_b sin),  y_b = amplitude (x_a sin + x_b cos),  angle = 2 pi frac(position * turns[i])
 // with (a, b) = (i, i + rot/2) or, interleaved, (2i, 2i + 1); columns from rot on are copied.  The inverse turns by the
 // negative angle: it is the transposed map, so it is also the gradient.
+//
+// Bound: HBM, every element read and written once.  A workgroup takes a few tokens: it forms their cosines and sines once
+// (64-bit reduction, one angle per pair and token) in LDS, then turns all query and key heads of those tokens, and in the
+// appending form copies the values, in pieces of four columns (eight with the partner columns of the half layout).
 #include "common.h"
+
+#include <algorithm>
 
 #include <cmath>
 
@@ -25,6 +31,9 @@ __device__ __forceinline__ void turn(const double turns, const long long positio
     s = k >= 2 ? -b : b;
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 struct RotaryArgs {
     int B, L, H, Hkv, d, rot;
     const double *turns;
@@ -34,62 +43,123 @@ struct RotaryArgs {
     float amplitude;
     int interleaved, inverse, token_major;
     long long Tcap;            // append only
+    int tokens, per_wg;        // B * L, tokens of a workgroup
 };
 
 __device__ __forceinline__ long long element(const RotaryArgs &a, const int heads, const int b, const int l, const int h) {
     return a.token_major ? (((long long)b * a.L + l) * heads + h) * a.d : (((long long)b * heads + h) * a.L + l) * a.d;
 }
 
-// One thread per (token, head, pair or copied column); APPEND writes the turned keys and the values into cache rows.
-template <bool APPEND>
+// VEC: pieces of four columns (d and rot multiples of 4, in the half layout rot a multiple of 8, rows on 16 bytes); otherwise a
+// piece is one pair, or one column that is copied.
+template <bool APPEND, bool VEC>
 __global__ __launch_bounds__(256) void rotary_f32(const float *q, float *q_out, const float *k, float *k_out, const float *v,
-                                                   float *v_out, RotaryArgs a, long long n) {
-    const int heads = a.H + a.Hkv, half = a.rot / 2, per = half + (a.d - a.rot);
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
-        const int c = (int)(e % per);
-        long long t = e / per;
-        const int h = (int)(t % heads);
-        t /= heads;
-        const int l = (int)(t % a.L), b = (int)(t / a.L);
-        long long pos = a.position0 + l;
-        if (a.positions) pos = APPEND ? (long long)a.positions[b] + l : a.positions[(long long)b * a.L + l];
-        const bool key = h >= a.H;
-        const float *x = key ? k + element(a, a.Hkv, b, l, h - a.H) : q + element(a, a.H, b, l, h);
-        float *y = key ? k_out + element(a, a.Hkv, b, l, h - a.H) : q_out + element(a, a.H, b, l, h);
-        if (APPEND && key) {
-            if (pos < 0 || pos >= a.Tcap || (a.counts && l >= a.counts[b])) continue;
-            y = k_out + (((long long)b * a.Hkv + (h - a.H)) * a.Tcap + pos) * a.d;
-        }
-        if (c < half) {
-            const int i = a.interleaved ? 2 * c : c, j = a.interleaved ? 2 * c + 1 : c + half;
-            float co, si;
-            turn(a.turns[c], pos, co, si);
-            co *= a.amplitude;
-            si *= a.inverse ? -a.amplitude : a.amplitude;
-            const float xa = x[i], xb = x[j];
-            y[i] = xa * co - xb * si;
-            y[j] = xa * si + xb * co;
+                                                   float *v_out, const RotaryArgs a) {
+    extern __shared__ __align__(16) f32x2 rotary_lds[];                    // [token][pair] cosine, sine
+    const int half = a.rot / 2, t0 = blockIdx.x * a.per_wg, nt = min(a.per_wg, a.tokens - t0);
+    auto position = [&](const int t) -> long long {                        // of token t = b L + l
+        if (!a.positions) return a.position0 + t % a.L;
+        return APPEND ? (long long)a.positions[t / a.L] + t % a.L : a.positions[t];
+    };
+    for (int e = threadIdx.x; e < nt * half; e += 256) {
+        float c, s;
+        turn(a.turns[e % half], position(t0 + e / half), c, s);
+        rotary_lds[e] = f32x2{c * a.amplitude, a.inverse ? -s * a.amplitude : s * a.amplitude};
+    }
+    __syncthreads();
+    // pieces of a head: those that turn, then those that are copied; of a token: the heads', then (append) the values'
+    const int turned = VEC ? (a.interleaved ? a.rot / 4 : a.rot / 8) : half;
+    const int piece = turned + (VEC ? (a.d - a.rot) / 4 : a.d - a.rot), values = APPEND ? (VEC ? a.d / 4 : a.d) : 0;
+    const int turning = (a.H + a.Hkv) * piece, all = turning + a.Hkv * values;
+    const bool in_place = !APPEND && q == q_out && k == k_out;
+    for (int e = threadIdx.x; e < nt * all; e += 256) {
+        // head-major tensors: the tokens of one head lie together, so they are the inner index over a head's pieces
+        int tt, i, h;
+        bool value = false;
+        if (a.token_major) {
+            tt = e / all;
+            i = e % all;
+            if (APPEND && i >= turning) { value = true; i -= turning; h = a.H + i / values; i %= values; }
+            else { h = i / piece; i %= piece; }
         } else {
-            y[a.rot + c - half] = x[a.rot + c - half];
+            i = e;
+            if (APPEND && i >= nt * turning) { value = true; i -= nt * turning; h = a.H + i / (nt * values); i %= nt * values; tt = i / values; i %= values; }
+            else { h = i / (nt * piece); i %= nt * piece; tt = i / piece; i %= piece; }
         }
+        const int t = t0 + tt, b = t / a.L, l = t % a.L;
+        const bool key = h >= a.H;
+        const int hh = key ? h - a.H : h;
+        const long long at = element(a, key ? a.Hkv : a.H, b, l, hh);
+        long long to = at;
         if (APPEND && key) {
-            const float *vx = v + element(a, a.Hkv, b, l, h - a.H);
-            float *vy = v_out + (((long long)b * a.Hkv + (h - a.H)) * a.Tcap + pos) * a.d;
-            if (c < half) {
-                vy[c] = vx[c];
-                vy[c + half] = vx[c + half];
+            const long long pos = position(t);
+            if (pos < 0 || pos >= a.Tcap || (a.counts && l >= a.counts[b])) continue;
+            to = (((long long)b * a.Hkv + hh) * a.Tcap + pos) * a.d;
+        }
+        const float *x = (value ? v : (key ? k : q)) + at;
+        float *y = (value ? v_out : (key ? k_out : q_out)) + to;
+        if (value || i >= turned) {
+            const int c = value ? i : (i - turned);
+            if (VEC) {
+                const int at4 = (value ? 0 : a.rot) + 4 * c;
+                if (!in_place) *reinterpret_cast<f32x4 *>(y + at4) = *reinterpret_cast<const f32x4 *>(x + at4);
             } else {
-                vy[a.rot + c - half] = vx[a.rot + c - half];
+                y[(value ? 0 : a.rot) + c] = x[(value ? 0 : a.rot) + c];
             }
+            continue;
+        }
+        const f32x2 *cs = rotary_lds + tt * half;
+        if (VEC && a.interleaved) {
+            const f32x4 z = *reinterpret_cast<const f32x4 *>(x + 4 * i);
+            const f32x2 u = cs[2 * i], w = cs[2 * i + 1];
+            *reinterpret_cast<f32x4 *>(y + 4 * i) = f32x4{z.x * u.x - z.y * u.y, z.x * u.y + z.y * u.x, z.z * w.x - z.w * w.y, z.z * w.y + z.w * w.x};
+        } else if (VEC) {
+            const f32x4 xa = *reinterpret_cast<const f32x4 *>(x + 4 * i), xb = *reinterpret_cast<const f32x4 *>(x + half + 4 * i);
+            f32x4 ya, yb;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const f32x2 u = cs[4 * i + c];
+                ya[c] = xa[c] * u.x - xb[c] * u.y;
+                yb[c] = xa[c] * u.y + xb[c] * u.x;
+            }
+            *reinterpret_cast<f32x4 *>(y + 4 * i) = ya;
+            *reinterpret_cast<f32x4 *>(y + half + 4 * i) = yb;
+        } else {
+            const int ca = a.interleaved ? 2 * i : i, cb = a.interleaved ? 2 * i + 1 : i + half;
+            const float xa = x[ca], xb = x[cb];
+            const f32x2 u = cs[i];
+            y[ca] = xa * u.x - xb * u.y;
+            y[cb] = xa * u.y + xb * u.x;
         }
     }
+}
+
+constexpr int MAX_ROTARY_DIM = 4096;       // a token's cosines and sines: 16 KiB of LDS
+
+template <bool APPEND>
+int launch_rotary(dl4s_hip_ctx *ctx, const float *q, float *q_out, const float *k, float *k_out, const float *v, float *v_out, RotaryArgs &a) {
+    uintptr_t bits = 0;
+    for (const void *p : {(const void *)q, (const void *)q_out, (const void *)k, (const void *)k_out, (const void *)v, (const void *)v_out})
+        bits |= reinterpret_cast<uintptr_t>(p);
+    const bool vec = (bits & 15) == 0 && a.d % 4 == 0 && a.rot % (a.interleaved ? 4 : 8) == 0;
+    // about 8192 columns a workgroup, while there are four workgroups to a compute unit, and at most 32 KiB of LDS
+    const int columns = (a.H + a.Hkv) * a.d;
+    a.tokens = a.B * a.L;
+    a.per_wg = std::max(1, std::min(8192 / columns, a.tokens / (4 * ctx->cu_count)));
+    if (a.rot) a.per_wg = std::max(1, std::min(a.per_wg, 32768 / (a.rot * 4)));
+    const size_t lds = (size_t)a.per_wg * (a.rot / 2) * sizeof(f32x2);
+    const dim3 grid((a.tokens + a.per_wg - 1) / a.per_wg);
+    if (vec) hipLaunchKernelGGL((rotary_f32<APPEND, true>), grid, dim3(256), lds, ctx->stream, q, q_out, k, k_out, v, v_out, a);
+    else hipLaunchKernelGGL((rotary_f32<APPEND, false>), grid, dim3(256), lds, ctx->stream, q, q_out, k, k_out, v, v_out, a);
+    return dl4s::launch_status("rotary_f32");
 }
 
 int rotary_checks(const char *what, int64_t B, int64_t L, int64_t H, int64_t Hkv, int64_t d, int64_t rot_dim, int64_t position0,
                   uint32_t flags, uint32_t known) {
     DL4S_REQUIRE(B >= 0 && L >= 0 && H >= 0 && Hkv >= 0, DL4S_HIP_EINVALID_ARG, "%s: negative extent", what);
     DL4S_REQUIRE(!(flags & ~known), DL4S_HIP_EINVALID_ARG, "%s: unknown flags %#x", what, flags);
-    DL4S_REQUIRE(d >= 1 && d <= (int64_t(1) << 20), DL4S_HIP_EUNSUPPORTED, "%s: head dim %lld", what, (long long)d);
+    DL4S_REQUIRE(d >= 1 && d <= MAX_ROTARY_DIM, DL4S_HIP_EUNSUPPORTED, "%s: head dim %lld (1 to %d are implemented)", what, (long long)d,
+                 MAX_ROTARY_DIM);
     DL4S_REQUIRE(rot_dim >= 0 && rot_dim <= d && rot_dim % 2 == 0, DL4S_HIP_ESHAPE, "%s: %lld turned columns of %lld (an even number is needed)", what,
                  (long long)rot_dim, (long long)d);
     const int64_t big = int64_t(1) << 30;
@@ -135,16 +205,12 @@ int dl4s_hip_rotary_f32(dl4s_hip_ctx *ctx, const float *q, float *q_out, const f
     const int rc = rotary_checks("rotary", B, L, H, Hkv, d, rot_dim, position0, flags,
                                  DL4S_ROTARY_INTERLEAVED | DL4S_ROTARY_INVERSE | DL4S_ROTARY_TOKEN_MAJOR);
     if (rc) return rc;
-    const long long n = (long long)B * L * (H + Hkv) * (rot_dim / 2 + (d - rot_dim));
-    if (n == 0) return DL4S_HIP_OK;
+    if (B * L == 0 || H + Hkv == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE((H == 0 || (q && q_out)) && (Hkv == 0 || (k && k_out)) && (rot_dim == 0 || turns), DL4S_HIP_EINVALID_ARG,
                  "rotary: NULL pointer");
-    const RotaryArgs a = {(int)B, (int)L, (int)H, (int)Hkv, (int)d, (int)rot_dim, turns, positions, position0, nullptr, amplitude,
-                          (flags & DL4S_ROTARY_INTERLEAVED) != 0, (flags & DL4S_ROTARY_INVERSE) != 0, (flags & DL4S_ROTARY_TOKEN_MAJOR) != 0, 0};
-    const long long blocks = (n + 255) / 256;
-    hipLaunchKernelGGL((rotary_f32<false>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, ctx->stream, q, q_out, k, k_out,
-                       (const float *)nullptr, (float *)nullptr, a, n);
-    return dl4s::launch_status("rotary_f32");
+    RotaryArgs a = {(int)B, (int)L, (int)H, (int)Hkv, (int)d, (int)rot_dim, turns, positions, position0, nullptr, amplitude,
+                    (flags & DL4S_ROTARY_INTERLEAVED) != 0, (flags & DL4S_ROTARY_INVERSE) != 0, (flags & DL4S_ROTARY_TOKEN_MAJOR) != 0, 0, 0, 0};
+    return launch_rotary<false>(ctx, H ? q : nullptr, H ? q_out : nullptr, Hkv ? k : nullptr, Hkv ? k_out : nullptr, nullptr, nullptr, a);
 }
 
 int dl4s_hip_rotary_append_f32(dl4s_hip_ctx *ctx, const float *q, const float *k_new, const float *v_new, float *q_out, float *kcache,
@@ -156,16 +222,13 @@ int dl4s_hip_rotary_append_f32(dl4s_hip_ctx *ctx, const float *q, const float *k
                                  DL4S_ROTARY_INTERLEAVED | DL4S_ROTARY_TOKEN_MAJOR);
     if (rc) return rc;
     DL4S_REQUIRE(Tcap >= 0 && Tcap < (int64_t(1) << 30), DL4S_HIP_EUNSUPPORTED, "rotary_append: cache capacity %lld", (long long)Tcap);
-    const long long n = (long long)B * L * (H + Hkv) * (rot_dim / 2 + (d - rot_dim));
-    if (n == 0) return DL4S_HIP_OK;
+    if (B * L == 0 || H + Hkv == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE((H == 0 || (q && q_out)) && (Hkv == 0 || (k_new && v_new && kcache && vcache)) && (rot_dim == 0 || turns),
                  DL4S_HIP_EINVALID_ARG, "rotary_append: NULL pointer");
-    const RotaryArgs a = {(int)B, (int)L, (int)H, (int)Hkv, (int)d, (int)rot_dim, turns, positions, position0, counts, amplitude,
-                          (flags & DL4S_ROTARY_INTERLEAVED) != 0, 0, (flags & DL4S_ROTARY_TOKEN_MAJOR) != 0, Tcap};
-    const long long blocks = (n + 255) / 256;
-    hipLaunchKernelGGL((rotary_f32<true>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, ctx->stream, q, q_out, k_new,
-                       kcache, v_new, vcache, a, n);
-    return dl4s::launch_status("rotary_f32");
+    RotaryArgs a = {(int)B, (int)L, (int)H, (int)Hkv, (int)d, (int)rot_dim, turns, positions, position0, counts, amplitude,
+                    (flags & DL4S_ROTARY_INTERLEAVED) != 0, 0, (flags & DL4S_ROTARY_TOKEN_MAJOR) != 0, Tcap, 0, 0};
+    return launch_rotary<true>(ctx, H ? q : nullptr, H ? q_out : nullptr, Hkv ? k_new : nullptr, Hkv ? kcache : nullptr, Hkv ? v_new : nullptr,
+                               Hkv ? vcache : nullptr, a);
 }
 
 }  // extern "C"

@@ -10,6 +10,7 @@
 #include <initializer_list>
 
 #include "sdpa_window_bwd.h"
+#include "sdpa_window_few.h"
 
 namespace {
 
@@ -226,10 +227,10 @@ WindowGeometry geometry(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t L
 
 // Kernels with more than 64 KiB of LDS have their limit raised once per device.
 template <typename K>
-int lds_limit(dl4s_hip_ctx *ctx, int kind, K kernel, size_t bytes) {
-    if (bytes > 65536 && dl4s::lds_limit_pending(ctx, dl4s::LDS_WINDOW, kind)) {
+int lds_limit(dl4s_hip_ctx *ctx, int family, int kind, K kernel, size_t bytes) {
+    if (bytes > 65536 && dl4s::lds_limit_pending(ctx, family, kind)) {
         DL4S_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        dl4s::lds_limit_done(ctx, dl4s::LDS_WINDOW, kind);
+        dl4s::lds_limit_done(ctx, family, kind);
     }
     return DL4S_HIP_OK;
 }
@@ -237,9 +238,8 @@ int lds_limit(dl4s_hip_ctx *ctx, int kind, K kernel, size_t bytes) {
 template <int DT, int BN>
 int launch_fwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, const WindowGeometry &g) {
     typedef Tile<BN, DT> T;
-    const size_t lds = 2 * 3 * (T::ROWS_PLANE + T::COLS_PLANE);
-    const int rc = lds_limit(ctx, DT / 32 - 1, sdpa_window_fwd_f32<DT, BN>, lds);
-    if (rc) return rc;
+    constexpr size_t lds = 2 * 3 * (T::ROWS_PLANE + T::COLS_PLANE);
+    static_assert(lds <= 65536, "more LDS needs its limit raised");
     hipLaunchKernelGGL((sdpa_window_fwd_f32<DT, BN>), dim3(8 * g.per_xcd), dim3(256), lds, ctx->stream, q, k, v, out, stats, g);
     return dl4s::launch_status("sdpa_window_fwd_f32");
 }
@@ -275,8 +275,8 @@ int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v
                float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
     typedef Tile<32, DT> T;
     const size_t lds_q = 2 * 3 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 3 * (2 * T::ROWS_PLANE + 2 * T::COLS_PLANE) + 96 * sizeof(float);
-    int rc = lds_limit(ctx, DT / 32 - 1, sdpa_window_dq_f32<DT>, lds_q);
-    if (!rc) rc = lds_limit(ctx, 4 + DT / 32 - 1, sdpa_window_dkv_f32<DT>, lds_k);
+    int rc = lds_limit(ctx, dl4s::LDS_WINDOW, DT / 32 - 1, sdpa_window_dq_f32<DT>, lds_q);
+    if (!rc) rc = lds_limit(ctx, dl4s::LDS_WINDOW, 4 + DT / 32 - 1, sdpa_window_dkv_f32<DT>, lds_k);
     if (rc) return rc;
     if (g.units) {
         hipLaunchKernelGGL((sdpa_window_dq_f32<DT>), dim3(8 * g.per_xcd), dim3(256), lds_q, ctx->stream, q, k, v, out, stats, dout, dq, delta, g);
@@ -295,6 +295,51 @@ int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v
         }
     }
     return rc;
+}
+
+// Few query rows: the workgroups and the split of the keys.  Lk is the number of rows that can be visible at all (T of a cache).
+template <int DT, int NW>
+int launch_few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, FewArgs &a, int64_t pairs) {
+    const int most_cols = std::min(16, a.cols);
+    const size_t lds = (size_t)NW * most_cols * (DT + 4) * sizeof(float);
+    const int rc = lds_limit(ctx, dl4s::LDS_WINDOW_FEW, DT == 64 ? 0 : (DT == 128 ? 1 : 2), sdpa_window_few_f32<DT, NW>, lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((sdpa_window_few_f32<DT, NW>), dim3(a.nsplit, (unsigned)pairs, (a.cols + 15) / 16), dim3(NW * 64), lds, ctx->stream, q, k,
+                       v, out, stats, a);
+    return dl4s::launch_status("sdpa_window_few_f32");
+}
+
+int few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, int64_t B, int64_t H, int64_t Hkv,
+             int64_t Lq, int64_t Lk, int64_t d, float rT, const WindowArgs &w, Layout lq, Layout lk) {
+    FewArgs a;
+    a.H = (int)H; a.Hkv = (int)Hkv; a.group = (int)(H / Hkv); a.Lq = (int)Lq; a.Lk = (int)Lk; a.d = (int)d;
+    a.cols = a.group * a.Lq;
+    a.rT = rT;
+    a.vec = d % 4 == 0 && on_16_bytes({q, k, v});
+    a.lq = lq; a.lk = lk; a.w = w;
+    const int64_t pairs = B * Hkv;
+    // Workgroups of 8 wavefronts.  Enough of them that every compute unit has one; a split costs a second launch, so up to
+    // 512 keys one workgroup reads them all, and a workgroup has at least 256 keys.
+    const int NW = 8;
+    const int64_t most = std::min<int64_t>(Lk, (int64_t)w.window + Lq - 1 + w.sinks), blocks = pairs * ((a.cols + 15) / 16);
+    int64_t ns = most <= 512 ? 1 : std::min((ctx->cu_count + blocks - 1) / blocks, (most + 255) / 256);
+    a.chunk = (int)std::max<int64_t>(16, ((most + ns - 1) / ns + 15) / 16 * 16);
+    a.nsplit = (int)std::max<int64_t>(1, (most + a.chunk - 1) / a.chunk);
+    a.partial = nullptr;
+    std::unique_lock<std::mutex> scratch_lock(ctx->scratch_mu, std::defer_lock);
+    int rc;
+    if (a.nsplit > 1) {
+        scratch_lock.lock();
+        rc = dl4s::ensure_scratch(ctx, (size_t)pairs * a.nsplit * a.cols * (d + 2) * sizeof(float));
+        if (rc) return rc;
+        a.partial = reinterpret_cast<float *>(ctx->scratch);
+    }
+    if (d <= 64) rc = launch_few_rows<64, NW>(ctx, q, k, v, out, stats, a, pairs);
+    else if (d <= 128) rc = launch_few_rows<128, NW>(ctx, q, k, v, out, stats, a, pairs);
+    else rc = launch_few_rows<256, NW>(ctx, q, k, v, out, stats, a, pairs);
+    if (rc || a.nsplit == 1) return rc;
+    hipLaunchKernelGGL(sdpa_window_merge_f32, dim3(a.cols, (unsigned)pairs), dim3(256), 0, ctx->stream, out, stats, a);
+    return dl4s::launch_status("sdpa_window_merge_f32");
 }
 
 // What the three entry points check alike.  Returns a status; *w is filled in.
@@ -336,6 +381,9 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     if (rows == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE(q && out && (Lk == 0 || (k && v)), DL4S_HIP_EINVALID_ARG, "sdpa_window_fwd: NULL tensor pointer");
     const bool tm = flags & DL4S_SDPA_TOKEN_MAJOR;
+    // few rows to a key head: the matrix kernels' tiles of 32 rows would be mostly empty, and their keys are not split
+    if (H / Hkv * Lq <= 32 && B * Hkv <= 65535)
+        return few_rows(ctx, q, k, v, out, stats, B, H, Hkv, Lq, Lk, d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d));
     if (d <= 128) {
         const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, on_16_bytes({q, k, v, out}), w);
         if (d <= 32) return launch_fwd<32, 64>(ctx, q, k, v, out, stats, g);
@@ -400,14 +448,14 @@ int dl4s_hip_sdpa_window_decode_f32(dl4s_hip_ctx *ctx, const float *q, const flo
     WindowArgs w;
     const int rc = window_checks("sdpa_window_decode", B, H, Hkv, 1, Tcap, d, &desc, 0, &w);
     if (rc) return rc;
-    const long long rows = (long long)B * H;
-    if (rows == 0) return DL4S_HIP_OK;
+    if (B * H == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE(q && kcache && vcache && out, DL4S_HIP_EINVALID_ARG, "sdpa_window_decode: NULL tensor pointer");
     DL4S_REQUIRE(T >= 1 && T <= Tcap, DL4S_HIP_ESHAPE, "sdpa_window_decode: T=%lld must be in [1, Tcap=%lld]", (long long)T, (long long)Tcap);
+    DL4S_REQUIRE(B * Hkv <= 65535 && H / Hkv <= (1 << 20), DL4S_HIP_EUNSUPPORTED,
+                 "sdpa_window_decode: B*Hkv=%lld above 65535, or more than 2^20 query heads to a key head", (long long)(B * Hkv));
     w.last_key = 1;
-    hipLaunchKernelGGL(sdpa_window_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, kcache, vcache, out, (float *)nullptr, (int)H,
-                       (int)(H / Hkv), 1, (int)T, (int)d, inv_temperature, w, layout(false, H, 1, d), layout(false, Hkv, Tcap, d), rows);
-    return dl4s::launch_status("sdpa_window_rows_f32");
+    return few_rows(ctx, q, kcache, vcache, out, nullptr, B, H, Hkv, 1, T, d, inv_temperature, w, layout(false, H, 1, d),
+                    layout(false, Hkv, Tcap, d));
 }
 
 }  // extern "C"

@@ -4,103 +4,304 @@
 //   m = max z,  L = log sum exp(z - m),  log p_j = (z_j - m) - L,  entropy = L - sum exp(z_j - m) (z_j - m) / sum exp(z - m)
 //   d(log p_t)/dz_j = [j = t] - p_j,  d(entropy)/dz_j = -p_j (log p_j + entropy)
 // A term of weight zero adds nothing to the entropy (z_j = -inf: a blocked token).
+//
+// Bound: reading the logits once from HBM (the gradient: reading and writing them once).  token_logprobs_f32 makes one pass:
+// every lane keeps a running maximum m, l = sum exp(z - m) and u = sum exp(z - m) (z - m) of its own values, in fp32, and a
+// wavefront keeps the alternatives as one sorted list, the i-th best in lane i.  A value and its token are one 64-bit
+// integer that orders them, so the list is exact and does not depend on who was ready first.  After the first tile few
+// values beat the k-th best (about k ln(n / 1024) of n in random order), each is found by a ballot and inserted by shifting
+// the lanes behind it; the wavefronts of a workgroup share the highest k-th best found so far.
 #include "common.h"
+
+#include <algorithm>
 
 namespace {
 
 constexpr int MAX_TOP = 64;
+constexpr int MERGE_KEYS = 1024;     // alternatives that one merge ranks
+constexpr float LOG2E = 1.44269504088896340736f;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64;
 
 __device__ __forceinline__ float scaled(const float x, const float t) { return x * t + 0.0f; }   // + 0: the two zeros are one value
+__device__ __forceinline__ float exp_fast(const float y) { return __builtin_amdgcn_exp2f(y * LOG2E); }
 
-// The order of the alternatives as one integer: larger value first, of equal values the lower token; NaN behind -inf.
-__device__ __forceinline__ unsigned long long order_key(const float z, const unsigned token) {
+// The order of the alternatives as one integer: larger value first, of equal values the lower token; NaN behind -inf.  0 is no token.
+__device__ __forceinline__ u64 order_key(const float z, const unsigned token) {
     unsigned u = __float_as_uint(z);
     u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
     if (z != z) u = 0;
-    return ((unsigned long long)u << 32) | (0xFFFFFFFFu - token);
+    return ((u64)u << 32) | (0xFFFFFFFFu - token);
+}
+__device__ __forceinline__ float key_value(const u64 key) {
+    const unsigned u = (unsigned)(key >> 32);
+    if (u == 0) return __builtin_nanf("");
+    return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+}
+__device__ __forceinline__ int key_token(const u64 key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
+
+__device__ __forceinline__ u64 lane_key(const u64 key, const int lane) {
+    return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)key, lane);
+}
+__device__ __forceinline__ u64 key_before(const u64 key) {       // the key of the lane before (lane 0: its own)
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp((int)(unsigned)key, (int)(unsigned)key, 0x138, 0xF, 0xF, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp((int)(key >> 32), (int)(key >> 32), 0x138, 0xF, 0xF, false);
+    return ((u64)hi << 32) | lo;
 }
 
-__device__ __forceinline__ float block_reduce(float v, float *sm, const bool max) {
-    for (int o = 32; o; o >>= 1) {
-        const float w = __shfl_xor(v, o, 64);
-        v = max ? fmaxf(v, w) : v + w;
-    }
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sm[0];
-    for (int w = 1; w < 4; ++w) v = max ? fmaxf(v, sm[w]) : v + sm[w];
-    __syncthreads();
+// Running maximum and sums of one lane, wavefront or part of a row.
+struct Sums {
+    float m, l, u;
+};
+__device__ __forceinline__ Sums rescaled(const Sums s, const float M) {      // s with M in place of its maximum
+    const float f = s.m == -INFINITY ? 0.f : exp_fast(s.m - M), d = s.m == -INFINITY ? 0.f : s.m - M;
+    Sums r;
+    r.m = M;
+    r.l = s.m == -INFINITY ? s.l : s.l * f;
+    r.u = s.m == -INFINITY ? s.u : f * (s.u + s.l * d);
+    return r;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
 
-// One workgroup per row: maximum, sums, then the alternatives one by one (the largest key below the last one).
-__global__ __launch_bounds__(256) void token_logprobs_f32(const float *__restrict__ x, long long n, long long stride, float t,
-                                                           const int *__restrict__ targets, int ignore, float *__restrict__ logprobs,
-                                                           float *__restrict__ entropy, float *__restrict__ stats, int top,
-                                                           float *__restrict__ top_logprobs, int *__restrict__ top_tokens) {
-    __shared__ float sm[4];
-    __shared__ unsigned long long sk[4];
-    const long long row = blockIdx.x;
-    const float *xr = x + row * stride;
-    const int tid = threadIdx.x;
-    float m = -INFINITY;
-    bool nan = false;
-    for (long long j = tid; j < n; j += 256) { const float z = scaled(xr[j], t); m = fmaxf(m, z); nan |= z != z; }
-    m = block_reduce(m, sm, true);
-    if (__syncthreads_or(nan)) m = __builtin_nanf("");
-    float l = 0.f, u = 0.f;
-    for (long long j = tid; j < n; j += 256) {
-        const float y = scaled(xr[j], t) - m, e = expf(y);
-        l += e;
-        if (e != 0.f) u += e * y;
+// What a row's sums and alternatives become.
+struct Outputs {
+    const int *targets;
+    int ignore;
+    float *logprobs, *entropy, *stats, *top_logprobs;
+    int *top_tokens;
+    int top;
+};
+__device__ __forceinline__ void row_results(const Outputs &o, const long long row, const float *xr, const long long n, const float t,
+                                            const Sums s) {
+    const float L = logf(s.l), H = L - s.u / s.l;
+    if (o.targets) {
+        const int g = o.targets[row];
+        o.logprobs[row] = g == o.ignore ? 0.f : (g < 0 || g >= n ? __builtin_nanf("") : (scaled(xr[g], t) - s.m) - L);
     }
-    l = block_reduce(l, sm, false);
-    u = block_reduce(u, sm, false);
-    const float L = logf(l), H = L - u / l;
-    if (tid == 0) {
-        if (targets && logprobs) {
-            const int g = targets[row];
-            logprobs[row] = g == ignore ? 0.f : (g < 0 || g >= n ? __builtin_nanf("") : (scaled(xr[g], t) - m) - L);
+    if (o.entropy) o.entropy[row] = H;
+    if (o.stats) { o.stats[3 * row] = s.m; o.stats[3 * row + 1] = L; o.stats[3 * row + 2] = H; }
+}
+// The `top` largest of `count` keys in LDS (0 = none) as outputs, or as keys: each is put where its rank says.
+__device__ __forceinline__ void rank_keys(const u64 *keys, const int count, const int top, const Outputs *o, const long long row, const Sums s,
+                                          u64 *to) {
+    for (int e = threadIdx.x; e < count; e += blockDim.x) {
+        const u64 key = keys[e];
+        if (key == 0) continue;
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += keys[j] > key;
+        if (rank >= top) continue;
+        if (to) to[rank] = key;
+        else {
+            o->top_tokens[row * top + rank] = key_token(key);
+            o->top_logprobs[row * top + rank] = (key_value(key) - s.m) - logf(s.l);
         }
-        if (entropy) entropy[row] = H;
-        if (stats) { stats[3 * row] = m; stats[3 * row + 1] = L; stats[3 * row + 2] = H; }
-    }
-    unsigned long long below = ~0ull;
-    for (int i = 0; i < top; ++i) {
-        unsigned long long best = 0;
-        for (long long j = tid; j < n; j += 256) {
-            const unsigned long long key = order_key(scaled(xr[j], t), (unsigned)j);
-            if (key < below && key > best) best = key;
-        }
-        for (int o = 32; o; o >>= 1) { const unsigned long long w = __shfl_xor(best, o, 64); best = w > best ? w : best; }
-        if ((tid & 63) == 0) sk[tid >> 6] = best;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) best = sk[w] > best ? sk[w] : best;
-        __syncthreads();
-        if (tid == 0) {
-            const unsigned token = 0xFFFFFFFFu - (unsigned)best;
-            top_tokens[row * top + i] = (int)token;
-            top_logprobs[row * top + i] = (scaled(xr[token], t) - m) - L;
-        }
-        below = best;
     }
 }
 
-__global__ __launch_bounds__(256) void token_logprobs_bwd_f32(const float *x, long long n, long long stride, float t,
-                                                               const int *__restrict__ targets, int ignore,
+// One workgroup per row, or per part of a row (blockIdx.x); parts leave [top keys][m, l, u] in scratch for the merge.
+template <int NW, bool TOP>
+__global__ __launch_bounds__(NW * 64) void token_logprobs_f32(const float *__restrict__ x, const long long n, const long long stride,
+                                                               const float t, const Outputs out, const int parts, u64 *partial) {
+    __shared__ Sums sums[NW];
+    __shared__ u64 keys[TOP ? NW * MAX_TOP : 1], bar;
+    const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
+    const int part = blockIdx.x;
+    const float *xr = x + row * stride;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (TOP) {
+        if (threadIdx.x == 0) bar = 0;
+        __syncthreads();
+    }
+
+    // granules of 16 bytes: granule g holds elements 4 g - before .. + 3 of the row
+    const int before = (int)((reinterpret_cast<uintptr_t>(xr) >> 2) & 3);
+    const long long granules = (n + before + 3) / 4, share = ((granules + parts - 1) / parts + 255) / 256 * 256;
+    const long long g0 = part * share, g1 = min(granules, g0 + share);
+    const float *xg = xr - before;
+
+    Sums s = {-INFINITY, 0.f, 0.f};
+    u64 list = 0, tau = 0;
+    bool filled = false;
+    for (long long base = g0 + 256 * wave; base < g1; base += 256 * NW) {
+        float z[16];
+        if (4 * base >= before && 4 * (base + 256) - before <= n) {          // no granule is cut by the row's ends
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(xg + 4 * (base + 64 * i + lane)));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z[4 * i + c] = scaled(v[c], t);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const long long j = 4 * (base + 64 * i + lane) - before + c;
+                    z[4 * i + c] = j >= 0 && j < n ? scaled(xr[j], t) : -INFINITY;
+                }
+        }
+        float mx = z[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, z[e]);
+        const float M = fmaxf(s.m, mx);
+        const float mu = M == -INFINITY ? 0.f : M;
+        s = rescaled(s, M);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float y = z[e] - mu, p = exp_fast(y);
+            s.l += p;
+            s.u += p * fmaxf(y, -1e4f);                                      // p = 0 far below: 0 * -inf is no term
+        }
+        if (TOP) {
+            // keys of the tile in registers again: a token outside the row has none
+            auto key_of = [&](const int e) {
+                const long long j = 4 * (base + 64 * (e >> 2) + lane) - before + (e & 3);
+                return j >= 0 && j < n ? order_key(z[e], (unsigned)j) : 0;
+            };
+            const u64 others = __hip_atomic_load(&bar, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            tau = others > tau ? others : tau;
+            // (tau below every value there is, NaN included, while its high word is 0)
+            if ((tau >> 32) == 0 || __any(mx >= key_value(tau))) {
+                unsigned taken = 0;                                          // the value of this lane that the list already holds
+                if (!filled) {
+                    // the first tile: every lane's best value, sorted by counting how many lanes have a better one
+                    filled = true;
+                    u64 best = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const u64 key = key_of(e);
+                        if (key > best) { best = key; taken = 1u << e; }
+                    }
+                    int rank = 0;
+#pragma unroll 16
+                    for (int i = 0; i < 64; ++i) {
+                        const u64 other = lane_key(best, i);
+                        rank += other > best || (other == best && i < lane);    // (equal only where there is no token)
+                    }
+                    const unsigned lo = (unsigned)__builtin_amdgcn_ds_permute(rank << 2, (int)(unsigned)best);
+                    const unsigned hi = (unsigned)__builtin_amdgcn_ds_permute(rank << 2, (int)(best >> 32));
+                    list = ((u64)hi << 32) | lo;
+                    const u64 kth = lane_key(list, out.top - 1);
+                    tau = kth > tau ? kth : tau;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const u64 key = (taken >> e) & 1 ? 0 : key_of(e);
+                    u64 better = __ballot(key > tau);
+                    while (better) {
+                        const int from = __builtin_ctzll(better);
+                        const u64 add = lane_key(key, from);
+                        const int pos = __popcll(__ballot(list > add));
+                        const u64 shifted = key_before(list);
+                        list = lane < pos ? list : (lane == pos ? add : shifted);
+                        const u64 kth = lane_key(list, out.top - 1);
+                        tau = kth > tau ? kth : tau;
+                        better &= __ballot(key > tau) & ~(1ull << from);
+                    }
+                }
+                if (lane == 0) __hip_atomic_fetch_max(&bar, tau, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+        }
+    }
+
+    const float M = wave_max(s.m);
+    s = rescaled(s, M);
+    s.l = dl4s::wave_sum(s.l);
+    s.u = dl4s::wave_sum(s.u);
+    if (lane == 0) sums[wave] = s;
+    if (TOP && lane < out.top) keys[wave * out.top + lane] = list;
+    __syncthreads();
+    float Mall = sums[0].m;
+#pragma unroll
+    for (int w = 1; w < NW; ++w) Mall = fmaxf(Mall, sums[w].m);
+    Sums all = rescaled(sums[0], Mall);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+        const Sums r = rescaled(sums[w], Mall);
+        all.l += r.l;
+        all.u += r.u;
+    }
+    u64 *rec = parts > 1 ? partial + (row * parts + part) * (out.top + 2) : nullptr;
+    if (threadIdx.x == 0) {
+        if (rec) {
+            float *f = reinterpret_cast<float *>(rec + out.top);
+            f[0] = all.m; f[1] = all.l; f[2] = all.u;
+        } else {
+            row_results(out, row, xr, n, t, all);
+        }
+    }
+    if (TOP) {
+        if (rec) {                     // a part may hold fewer keys than asked for
+            for (int e = threadIdx.x; e < out.top; e += NW * 64) rec[e] = 0;
+            __syncthreads();
+        }
+        rank_keys(keys, NW * out.top, out.top, &out, row, all, rec);
+    }
+}
+
+// Joins the parts of a row: one workgroup per row.
+__global__ __launch_bounds__(256) void token_logprobs_merge_f32(const float *__restrict__ x, const long long n, const long long stride,
+                                                                 const float t, const Outputs out, const int parts, const u64 *partial) {
+    __shared__ u64 keys[MERGE_KEYS];
+    const long long row = blockIdx.x;
+    const u64 *rec = partial + row * parts * (out.top + 2);
+    Sums all = {-INFINITY, 0.f, 0.f};
+    float M = -INFINITY;
+    for (int p = 0; p < parts; ++p) M = fmaxf(M, reinterpret_cast<const float *>(rec + p * (out.top + 2) + out.top)[0]);
+    for (int p = 0; p < parts; ++p) {
+        const float *f = reinterpret_cast<const float *>(rec + p * (out.top + 2) + out.top);
+        const Sums r = rescaled(Sums{f[0], f[1], f[2]}, M);
+        all.l += r.l;
+        all.u += r.u;
+    }
+    all.m = M;
+    if (threadIdx.x == 0) row_results(out, row, x + row * stride, n, t, all);
+    for (int e = threadIdx.x; e < parts * out.top; e += 256) keys[e] = rec[e / out.top * (out.top + 2) + e % out.top];
+    __syncthreads();
+    rank_keys(keys, parts * out.top, out.top, &out, row, all, nullptr);
+}
+
+// One workgroup per 4096 elements of a row.
+__global__ __launch_bounds__(256) void token_logprobs_bwd_f32(const float *x, const long long n, const long long stride, const float t,
+                                                               const int *__restrict__ targets, const int ignore,
                                                                const float *__restrict__ stats, const float *__restrict__ dlogprobs,
                                                                const float *__restrict__ dentropy, float *dx) {
-    const long long row = blockIdx.x;
+    const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
     const float m = stats[3 * row], L = stats[3 * row + 1], H = stats[3 * row + 2];
     const int g = targets ? targets[row] : ignore;
     const float gl = (dlogprobs && g != ignore) ? (g < 0 || g >= n ? __builtin_nanf("") : dlogprobs[row]) : 0.f;
     const float ge = dentropy ? dentropy[row] : 0.f;
-    for (long long j = threadIdx.x; j < n; j += 256) {
-        const float lp = (scaled(x[row * stride + j], t) - m) - L, p = expf(lp);
-        float r = -p * gl;
-        if (p != 0.f) r -= ge * p * (lp + H);
+    const float *xr = x + row * stride;
+    float *dr = dx + row * stride;
+    auto gradient = [&](const float v, const long long j) {
+        const float lp = (scaled(v, t) - m) - L, p = exp_fast(lp);
+        float r = -p * (gl + ge * (fmaxf(lp, -1e4f) + H));
         if (j == g) r += gl;
-        dx[row * stride + j] = r * t;
+        return r * t;
+    };
+    const int before = (int)((reinterpret_cast<uintptr_t>(xr) >> 2) & 3);
+    const bool alike = ((reinterpret_cast<uintptr_t>(dr) ^ reinterpret_cast<uintptr_t>(xr)) & 15) == 0;
+    const long long base = (long long)blockIdx.x * 1024;
+    if (alike && 4 * base >= before && 4 * (base + 1024) - before <= n) {
+        f32x4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(xr - before + 4 * (base + 256 * i + threadIdx.x)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long j = 4 * (base + 256 * i + threadIdx.x) - before;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[i][c] = gradient(v[i][c], j + c);
+            __builtin_nontemporal_store(v[i], reinterpret_cast<f32x4 *>(dr + j));
+        }
+    } else {
+        for (int i = 0; i < 16; ++i) {
+            const long long j = 4 * base - before + 256 * i + threadIdx.x;
+            if (j >= 0 && j < n) dr[j] = gradient(xr[j], j);
+        }
     }
 }
 
@@ -114,6 +315,17 @@ int logprob_checks(const char *what, int64_t rows, int64_t n, int64_t stride, co
     return DL4S_HIP_OK;
 }
 
+// Rows on the grid's second and third axis (65535 at most on the second).  The caller splits launches of partly filled layers.
+template <typename F>
+int over_rows(int64_t rows, F launch) {
+    const int64_t whole = rows / 65535 * 65535;
+    if (whole) {
+        const int rc = launch(int64_t(0), dim3(0, 65535, (unsigned)(whole / 65535)));
+        if (rc) return rc;
+    }
+    return rows > whole ? launch(whole, dim3(0, (unsigned)(rows - whole), 1)) : DL4S_HIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -122,7 +334,7 @@ int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t 
                                 float inv_temperature, const int32_t *targets, int32_t ignore_index, float *logprobs, float *entropy,
                                 float *stats, int64_t top_k, float *top_logprobs, int32_t *top_tokens) {
     DL4S_CHECK_CTX(ctx);
-    const int rc = logprob_checks("token_logprobs", rows, n, row_stride, logits);
+    int rc = logprob_checks("token_logprobs", rows, n, row_stride, logits);
     if (rc || rows == 0) return rc;
     DL4S_REQUIRE((targets != nullptr) == (logprobs != nullptr), DL4S_HIP_EINVALID_ARG,
                  "token_logprobs: targets and logprobs come together");
@@ -130,9 +342,44 @@ int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t 
                  (long long)top_k, MAX_TOP);
     DL4S_REQUIRE(top_k <= n, DL4S_HIP_ESHAPE, "token_logprobs: %lld alternatives of %lld tokens", (long long)top_k, (long long)n);
     DL4S_REQUIRE(top_k == 0 || (top_logprobs && top_tokens), DL4S_HIP_EINVALID_ARG, "token_logprobs: NULL output for the alternatives");
-    hipLaunchKernelGGL(token_logprobs_f32, dim3((unsigned)rows), dim3(256), 0, ctx->stream, logits, (long long)n, (long long)row_stride,
-                       inv_temperature, targets, ignore_index, logprobs, entropy, stats, (int)top_k, top_logprobs, top_tokens);
-    return dl4s::launch_status("token_logprobs_f32");
+    // Few rows: 16 wavefronts to a row, and long rows in parts of at least 16384 tokens (a wavefront's tile each) until every
+    // compute unit has one.  Many rows: 4 wavefronts, whose lists of alternatives are filled over longer pieces.
+    const bool few = rows <= ctx->cu_count;
+    int64_t parts = 1;
+    if (few) {
+        parts = std::min<int64_t>(n / 16384, ctx->cu_count / rows);
+        parts = std::min<int64_t>(parts, top_k ? MERGE_KEYS / top_k : 64);
+        parts = std::max<int64_t>(parts, 1);
+    }
+    std::unique_lock<std::mutex> scratch_lock(ctx->scratch_mu, std::defer_lock);
+    u64 *partial = nullptr;
+    if (parts > 1) {
+        scratch_lock.lock();
+        rc = dl4s::ensure_scratch(ctx, (size_t)rows * parts * (top_k + 2) * sizeof(u64));
+        if (rc) return rc;
+        partial = reinterpret_cast<u64 *>(ctx->scratch);
+    }
+    rc = over_rows(rows, [&](const int64_t from, dim3 grid) {
+        grid.x = (unsigned)parts;
+        const Outputs out = {targets ? targets + from : nullptr, ignore_index, logprobs ? logprobs + from : nullptr,
+                             entropy ? entropy + from : nullptr, stats ? stats + 3 * from : nullptr,
+                             top_k ? top_logprobs + from * top_k : nullptr, top_k ? top_tokens + from * top_k : nullptr, (int)top_k};
+        const float *x = logits + from * row_stride;
+#define DL4S_LOGPROBS(NW, TOP)                                                                                                     \
+    hipLaunchKernelGGL((token_logprobs_f32<NW, TOP>), grid, dim3(NW * 64), 0, ctx->stream, x, (long long)n, (long long)row_stride, \
+                       inv_temperature, out, (int)parts, partial)
+        if (few && top_k) DL4S_LOGPROBS(16, true);
+        else if (few) DL4S_LOGPROBS(16, false);
+        else if (top_k) DL4S_LOGPROBS(4, true);
+        else DL4S_LOGPROBS(4, false);
+#undef DL4S_LOGPROBS
+        return dl4s::launch_status("token_logprobs_f32");
+    });
+    if (rc || parts == 1) return rc;
+    const Outputs out = {targets, ignore_index, logprobs, entropy, stats, top_logprobs, top_tokens, (int)top_k};
+    hipLaunchKernelGGL(token_logprobs_merge_f32, dim3((unsigned)rows), dim3(256), 0, ctx->stream, logits, (long long)n, (long long)row_stride,
+                       inv_temperature, out, (int)parts, (const u64 *)partial);
+    return dl4s::launch_status("token_logprobs_merge_f32");
 }
 
 int dl4s_hip_token_logprobs_bwd_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t rows, int64_t n, int64_t row_stride,
@@ -143,9 +390,13 @@ int dl4s_hip_token_logprobs_bwd_f32(dl4s_hip_ctx *ctx, const float *logits, int6
     if (rc || rows == 0) return rc;
     DL4S_REQUIRE(stats && dlogits, DL4S_HIP_EINVALID_ARG, "token_logprobs_bwd: NULL pointer");
     DL4S_REQUIRE(!dlogprobs || targets, DL4S_HIP_EINVALID_ARG, "token_logprobs_bwd: a gradient of the log probabilities without targets");
-    hipLaunchKernelGGL(token_logprobs_bwd_f32, dim3((unsigned)rows), dim3(256), 0, ctx->stream, logits, (long long)n,
-                       (long long)row_stride, inv_temperature, targets, ignore_index, stats, dlogprobs, dentropy, dlogits);
-    return dl4s::launch_status("token_logprobs_bwd_f32");
+    return over_rows(rows, [&](const int64_t from, dim3 grid) {
+        grid.x = (unsigned)((n + 3 + 4095) / 4096);                    // (up to three elements of the first granule lie before the row)
+        hipLaunchKernelGGL(token_logprobs_bwd_f32, grid, dim3(256), 0, ctx->stream, logits + from * row_stride, (long long)n,
+                           (long long)row_stride, inv_temperature, targets ? targets + from : nullptr, ignore_index, stats + 3 * from,
+                           dlogprobs ? dlogprobs + from : nullptr, dentropy ? dentropy + from : nullptr, dlogits + from * row_stride);
+        return dl4s::launch_status("token_logprobs_bwd_f32");
+    });
 }
 
 }  // extern "C"
