@@ -209,8 +209,7 @@ inline bool on_16_bytes(std::initializer_list<const void *> ps) {
 }
 
 // Query heads of a group that one workgroup takes together, and the rest of the launch.
-WindowGeometry geometry(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float rT, bool token_major, bool aligned,
-                        const WindowArgs &w) {
+WindowGeometry geometry(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float rT, bool token_major, const WindowArgs &w) {
     WindowGeometry g;
     g.H = (int)H; g.Hkv = (int)Hkv; g.group = (int)(H / Hkv); g.Lq = (int)Lq; g.Lk = (int)Lk; g.d = (int)d;
     g.hp = g.group % 4 == 0 ? 4 : (g.group % 2 == 0 ? 2 : 1);
@@ -218,7 +217,6 @@ WindowGeometry geometry(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t L
     g.units = (int)(B * Hkv * (g.group / g.hp) * g.nqb);
     g.per_xcd = (g.units + 7) / 8;
     g.rT = rT;
-    g.vec = aligned && d % 4 == 0;
     g.lq = layout(token_major, H, Lq, d);
     g.lk = layout(token_major, Hkv, Lk, d);
     g.w = w;
@@ -235,13 +233,20 @@ int lds_limit(dl4s_hip_ctx *ctx, int family, int kind, K kernel, size_t bytes) {
     return DL4S_HIP_OK;
 }
 
-template <int DT, int BN>
+template <int DT, int BN, bool VEC>
 int launch_fwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, const WindowGeometry &g) {
     typedef Tile<BN, DT> T;
-    constexpr size_t lds = 2 * 3 * (T::ROWS_PLANE + T::COLS_PLANE);
+    constexpr size_t lds = 2 * 2 * (T::ROWS_PLANE + T::COLS_PLANE);
     static_assert(lds <= 65536, "more LDS needs its limit raised");
-    hipLaunchKernelGGL((sdpa_window_fwd_f32<DT, BN>), dim3(8 * g.per_xcd), dim3(256), lds, ctx->stream, q, k, v, out, stats, g);
+    hipLaunchKernelGGL((sdpa_window_fwd_f32<DT, BN, VEC>), dim3(8 * g.per_xcd), dim3(256), lds, ctx->stream, q, k, v, out, stats, g);
     return dl4s::launch_status("sdpa_window_fwd_f32");
+}
+template <bool VEC>
+int launch_fwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, const WindowGeometry &g) {
+    if (g.d <= 32) return launch_fwd<32, 64, VEC>(ctx, q, k, v, out, stats, g);
+    if (g.d <= 64) return launch_fwd<64, 64, VEC>(ctx, q, k, v, out, stats, g);
+    if (g.d <= 96) return launch_fwd<96, 32, VEC>(ctx, q, k, v, out, stats, g);
+    return launch_fwd<128, 32, VEC>(ctx, q, k, v, out, stats, g);
 }
 
 // Deals the key blocks to workgroups.  A block that every later query sees (first keys) gets about as many query tiles per
@@ -270,21 +275,21 @@ KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B
     return kb;
 }
 
-template <int DT>
+template <int DT, bool VEC>
 int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats, const float *dout,
                float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
     typedef Tile<32, DT> T;
-    const size_t lds_q = 2 * 3 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 3 * (2 * T::ROWS_PLANE + 2 * T::COLS_PLANE) + 96 * sizeof(float);
-    int rc = lds_limit(ctx, dl4s::LDS_WINDOW, DT / 32 - 1, sdpa_window_dq_f32<DT>, lds_q);
-    if (!rc) rc = lds_limit(ctx, dl4s::LDS_WINDOW, 4 + DT / 32 - 1, sdpa_window_dkv_f32<DT>, lds_k);
+    const size_t lds_q = 2 * 2 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 2 * (2 * T::ROWS_PLANE + 2 * T::COLS_PLANE);
+    int rc = lds_limit(ctx, dl4s::LDS_WINDOW, 2 * (DT / 32 - 1) + VEC, sdpa_window_dq_f32<DT, VEC>, lds_q);
+    if (!rc) rc = lds_limit(ctx, dl4s::LDS_WINDOW_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dkv_f32<DT, VEC>, lds_k);
     if (rc) return rc;
     if (g.units) {
-        hipLaunchKernelGGL((sdpa_window_dq_f32<DT>), dim3(8 * g.per_xcd), dim3(256), lds_q, ctx->stream, q, k, v, out, stats, dout, dq, delta, g);
+        hipLaunchKernelGGL((sdpa_window_dq_f32<DT, VEC>), dim3(8 * g.per_xcd), dim3(256), lds_q, ctx->stream, q, k, v, out, stats, dout, dq, delta, g);
         rc = dl4s::launch_status("sdpa_window_dq_f32");
         if (rc) return rc;
     }
     if (kb.pairs && kb.blocks) {
-        hipLaunchKernelGGL((sdpa_window_dkv_f32<DT>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1])), dim3(256), lds_k, ctx->stream, q, k, v, stats,
+        hipLaunchKernelGGL((sdpa_window_dkv_f32<DT, VEC>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1])), dim3(256), lds_k, ctx->stream, q, k, v, stats,
                            dout, delta, dk, dv, g, kb);
         rc = dl4s::launch_status("sdpa_window_dkv_f32");
         for (int c = 0; c < 2 && !rc; ++c) {
@@ -295,6 +300,15 @@ int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v
         }
     }
     return rc;
+}
+
+template <bool VEC>
+int launch_bwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats,
+                     const float *dout, float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
+    if (g.d <= 32) return launch_bwd<32, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+    if (g.d <= 64) return launch_bwd<64, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+    if (g.d <= 96) return launch_bwd<96, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+    return launch_bwd<128, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
 }
 
 // Few query rows: the workgroups and the split of the keys.  Lk is the number of rows that can be visible at all (T of a cache).
@@ -357,10 +371,12 @@ int window_checks(const char *what, int64_t B, int64_t H, int64_t Hkv, int64_t L
     const int64_t big = int64_t(1) << 30;
     DL4S_REQUIRE(Lq < big && Lk < big && B < big && H < big && B * H < big && desc->q_offset < big, DL4S_HIP_EUNSUPPORTED,
                  "%s: an extent or the offset above 2^30", what);
+    DL4S_REQUIRE(H * d <= (int64_t(1) << 22), DL4S_HIP_EUNSUPPORTED, "%s: %lld heads of %lld: a token's heads above 2^22 values", what,
+                 (long long)H, (long long)d);
     DL4S_REQUIRE(B * H * Lq < big * 4 && B * Hkv * Lk < big * 4, DL4S_HIP_EUNSUPPORTED, "%s: more than 2^32 rows", what);
     w->window = (int)(desc->window < big ? desc->window : big);
     w->sinks = (int)(desc->sinks < Lk ? desc->sinks : Lk);
-    w->q_offset = desc->q_offset;
+    w->q_offset = (int)desc->q_offset;
     w->lengths = desc->lengths;
     w->last_key = 0;
     return DL4S_HIP_OK;
@@ -385,11 +401,9 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     if (H / Hkv * Lq <= 32 && B * Hkv <= 65535)
         return few_rows(ctx, q, k, v, out, stats, B, H, Hkv, Lq, Lk, d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d));
     if (d <= 128) {
-        const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, on_16_bytes({q, k, v, out}), w);
-        if (d <= 32) return launch_fwd<32, 64>(ctx, q, k, v, out, stats, g);
-        if (d <= 64) return launch_fwd<64, 64>(ctx, q, k, v, out, stats, g);
-        if (d <= 96) return launch_fwd<96, 32>(ctx, q, k, v, out, stats, g);
-        return launch_fwd<128, 32>(ctx, q, k, v, out, stats, g);
+        const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
+        return d % 4 == 0 && on_16_bytes({q, k, v, out}) ? launch_fwd_width<true>(ctx, q, k, v, out, stats, g)
+                                                         : launch_fwd_width<false>(ctx, q, k, v, out, stats, g);
     }
     hipLaunchKernelGGL(sdpa_window_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, k, v, out, stats, (int)H, (int)(H / Hkv),
                        (int)Lq, (int)Lk, (int)d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d), rows);
@@ -413,16 +427,15 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     std::unique_lock<std::mutex> scratch_lock(ctx->scratch_mu);
     const size_t delta_bytes = ((size_t)rows * sizeof(float) + 255) / 256 * 256;
     if (d <= 128 && H > 0) {
-        const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, on_16_bytes({q, k, v, out, dout, dq, dk, dv}), w);
+        const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
         KeyBlocks kb = krows ? key_blocks(ctx, g, B) : KeyBlocks{};
         rc = dl4s::ensure_scratch(ctx, delta_bytes + reinterpret_cast<size_t>(kb.partial));
         if (rc) return rc;
         float *delta = reinterpret_cast<float *>(ctx->scratch);
         kb.partial = delta + delta_bytes / sizeof(float);
-        if (d <= 32) return launch_bwd<32>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
-        if (d <= 64) return launch_bwd<64>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
-        if (d <= 96) return launch_bwd<96>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
-        return launch_bwd<128>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+        return d % 4 == 0 && on_16_bytes({q, k, v, out, dout, dq, dk, dv})
+                   ? launch_bwd_width<true>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb)
+                   : launch_bwd_width<false>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
     }
     rc = dl4s::ensure_scratch(ctx, delta_bytes);
     if (rc) return rc;

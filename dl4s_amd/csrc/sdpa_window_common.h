@@ -1,12 +1,15 @@
-// Shared by the windowed attention kernels: which keys a query sees, and fp32 products on the bf16 matrix instructions.
+// Shared by the windowed attention kernels: which keys a query sees, and fp32 products on the fp16 matrix instructions.
 //
-// A value x is held as three bf16 planes, x = h + m + l: h = bf16(x), m = bf16(x - h), l = bf16(x - h - m), each rounded to
-// nearest, so that h, m, l carry 8 + 8 + 8 significant bits and what is dropped is below 2^-27 |x|.  A product is six matrix
-// instructions (l.h + h.l + m.m + m.h + h.m + h.h, the small ones first); the three left out are below 2^-25 |x y|, less than
-// the rounding of one fp32 product, and the accumulators are fp32.  Measured against 64 bits, sums of 64 products of normal
-// values are off by 1.2e-7 of their size this way, 1.5e-7 through v_mfma_f32_32x32x2_f32.  Why: a 32 x 32 x 16 step costs
-// 6 x 36 = 216 SIMD cycles (measured) where eight fp32 steps cost 8 x 66 = 525, and the vector ALU runs beside the bf16
-// instructions (up to six vector instructions per matrix instruction cost nothing), not beside the fp32 ones.
+// A value x is held as two fp16 planes of x times a power of two, x 2^a = h + l with h = fp16(x 2^a), l = fp16(x 2^a - h),
+// each rounded to nearest: 11 + 11 significant bits.  A product is three matrix instructions, l.h + h.l + h.h (the small ones
+// first), summed in fp32; the one left out is below 2^-22 of the product.  The power of two puts the largest finite value of
+// what shares it (a row for an operand in registers, the tiles seen so far for one in LDS) at 2^14 or more, so a value 2^28
+// times smaller still has all its bits, a smaller one an error of 2^-39 of that largest, and nothing overflows.  Measured
+// against 64 bits, sums of 64 (512) products of normal values are off by 1.2e-7 (2.5e-7) of their size this way, 1.5e-7
+// (3.8e-7) through v_mfma_f32_32x32x2_f32.  Why: a 32 x 32 x 16 step costs 3 x 39 SIMD cycles (measured) where eight fp32
+// steps cost 8 x 66, and the vector ALU runs beside the fp16 instructions, not beside the fp32 ones.  Three bf16 planes
+// need no power of two, but six instructions and half as much again of registers and LDS (the forward pass of B8 H16 L2048
+// d64 window 512 took 244 us that way).
 // An infinity has no such planes (inf - inf): it turns the sums it enters into NaN.
 #pragma once
 #include "common.h"
@@ -16,8 +19,8 @@ namespace {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16;
@@ -27,12 +30,16 @@ constexpr int MAXD = 256;
 
 __device__ __forceinline__ float exp2_fast(const float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Positions are below 2^31 (offset and extents below 2^30), so all comparisons are 32-bit.
 struct WindowArgs {
     int window, sinks;      // clamped to [1, 2^30] and [0, Lk]
-    long long q_offset;
+    int q_offset;
     const int *lengths;
     int last_key;           // decode: the query of batch element b stands at position lengths[b] - 1 (or Lk - 1)
 };
+__device__ __forceinline__ bool sees(const WindowArgs &w, const int p, const int j, const int len) {
+    return (j <= p) & (j < len) & ((j > p - w.window) | (j < w.sinks));
+}
 
 // The keys a query sees, as two ranges [0, first) and [lo, hi) with first <= lo.
 struct Range {
@@ -43,13 +50,11 @@ __device__ __forceinline__ int valid_keys(const WindowArgs &w, const int b, cons
     return len < 0 ? 0 : (len > Lk ? Lk : len);
 }
 __device__ __forceinline__ Range visible_keys(const WindowArgs &w, const int b, const int i, const int Lk) {
-    const int len = valid_keys(w, b, Lk);
-    const long long p = w.last_key ? (long long)len - 1 : w.q_offset + i;
+    const int len = valid_keys(w, b, Lk), p = w.last_key ? len - 1 : w.q_offset + i;
     Range r;
-    const long long lo = p - w.window + 1;
-    r.hi = (int)(p + 1 < len ? p + 1 : len);
-    r.lo = lo < 0 ? 0 : (int)(lo > r.hi ? r.hi : lo);
-    r.first = w.sinks < r.lo ? w.sinks : r.lo;
+    r.hi = min(p + 1, len);
+    r.lo = min(max(p - w.window + 1, 0), r.hi);
+    r.first = min(w.sinks, r.lo);
     return r;
 }
 
@@ -79,45 +84,136 @@ __device__ __forceinline__ void store4(float *row, const int col, const int d, c
     }
 }
 
+// ---- powers of two
+__device__ __forceinline__ float pow2(const int a) { return __builtin_ldexpf(1.0f, a); }
+// The power that puts m (>= 0, finite) into [2^14, 2^15); tiny m stop at 2^125, which is as good.
+__device__ __forceinline__ int scale_of(const float m) {
+    const int e = (int)(__float_as_uint(m) >> 23);
+    return 141 - min(max(e, 16), 254);
+}
+__device__ __forceinline__ float finite_abs(const float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+template <int CTRL>
+__device__ __forceinline__ float max_lanes(const float v) {
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)));
+}
+// Largest of the 64 lanes' values (>= 0), uniform.
+__device__ __forceinline__ float wave_max_abs(float v) {
+    v = max_lanes<0xB1>(v);
+    v = max_lanes<0x4E>(v);
+    v = max_lanes<0x141>(v);
+    v = max_lanes<0x140>(v);
+    const unsigned u = __float_as_uint(v);
+    const unsigned r0 = __builtin_amdgcn_readlane(u, 0), r1 = __builtin_amdgcn_readlane(u, 16), r2 = __builtin_amdgcn_readlane(u, 32),
+                   r3 = __builtin_amdgcn_readlane(u, 48);
+    return __uint_as_float(max(max(r0, r1), max(r2, r3)));
+}
+template <int N>
+__device__ __forceinline__ float largest(const f32x4 (&x)[N]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(fmaxf(m, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+    if (__any(!(m < INFINITY))) {      // infinities do not set the scale of their neighbours
+        m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(fmaxf(m, fmaxf(finite_abs(x[i].x), finite_abs(x[i].y))), fmaxf(finite_abs(x[i].z), finite_abs(x[i].w)));
+    }
+    return m;
+}
+
 // The planes of a pair of values, the first in the low half of each word.
 struct Planes {
-    unsigned h, m, l;
+    unsigned h, l;
 };
+// x minus the low / high half of h, one instruction each
+__device__ __forceinline__ float minus_low(const float x, const unsigned h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(x), "v"(h));
+    return r;
+}
+__device__ __forceinline__ float minus_high(const float x, const unsigned h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(x), "v"(h));
+    return r;
+}
 __device__ __forceinline__ unsigned round2(const float a, const float b) {
-    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf16x2));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
 __device__ __forceinline__ Planes split2(const float a, const float b) {
     Planes p;
     p.h = round2(a, b);
-    const float a1 = a - __uint_as_float(p.h << 16), b1 = b - __uint_as_float(p.h & 0xffff0000u);
-    p.m = round2(a1, b1);
-    p.l = round2(a1 - __uint_as_float(p.m << 16), b1 - __uint_as_float(p.m & 0xffff0000u));
+    p.l = round2(minus_low(a, p.h), minus_high(b, p.h));
     return p;
 }
 
 // One lane's share of an operand of a 32 x 32 x 16 step: eight values along the contraction, as planes.
 struct Frag {
-    bf16x8 h, m, l;
+    f16x8 h, l;
 };
 __device__ __forceinline__ Frag split8(const float (&x)[8]) {
-    u32x4 h, m, l;
+    u32x4 h, l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const Planes p = split2(x[2 * i], x[2 * i + 1]);
-        h[i] = p.h; m[i] = p.m; l[i] = p.l;
+        h[i] = p.h; l[i] = p.l;
     }
-    return Frag{__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, m), __builtin_bit_cast(bf16x8, l)};
+    return Frag{__builtin_bit_cast(f16x8, h), __builtin_bit_cast(f16x8, l)};
 }
-__device__ __forceinline__ f32x16 mma6(const Frag &a, const Frag &b, f32x16 c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.l, b.h, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.l, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.m, b.m, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.m, b.h, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.m, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.h, c, 0, 0, 0);
+__device__ __forceinline__ f32x16 mma3(const Frag &a, const Frag &b, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l, b.h, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.l, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
 }
 
-// Tiles of R rows x C columns in LDS as planes, written by a workgroup of 256 from fp32 rows in global memory.
+__device__ __forceinline__ float max_halves(const float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float sum_halves(const float v) { return v + __shfl_xor(v, 32, 64); }
+
+// A row of up to DT columns, one row per lane of a half wavefront (lane and lane ^ 32 share it), as the operand whose
+// contraction runs along the row; f0 and f1 are multiplied in one after the other.  Returns the row's power of two.
+template <int DT, typename Load>
+__device__ __forceinline__ int row_operand(Frag (&f)[DT / 16], const Load load, const float f0, const float f1) {
+    const int half = (threadIdx.x & 63) >> 5;
+    f32x4 x[DT / 8];
+#pragma unroll
+    for (int s = 0; s < DT / 16; ++s) {
+        x[2 * s] = load(16 * s + 8 * half);
+        x[2 * s + 1] = load(16 * s + 8 * half + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < DT / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = (x[i][e] * f0) * f1;
+    const int a = scale_of(max_halves(largest(x)));
+    const float p = pow2(a);
+#pragma unroll
+    for (int s = 0; s < DT / 16; ++s) {
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { z[e] = x[2 * s][e] * p; z[4 + e] = x[2 * s + 1][e] * p; }
+        f[s] = split8(z);
+    }
+    return a;
+}
+
+// Rows of a tile of fp32 tensors through a buffer descriptor made per tile: rows at or beyond the tensor's valid ones, and
+// columns at or beyond d (whose offset lies outside every descriptor), read as zeros without a branch.
+constexpr unsigned NOWHERE = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const float *base, const int stride, const int r0, const int rows, const int n,
+                                                            const int d) {
+    const int m = min(rows - r0, n);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(base + (long long)r0 * stride), 0, m > 0 ? ((m - 1) * stride + d) * 4 : 0, 0x00020000);
+}
+template <bool VEC>
+__device__ __forceinline__ f32x4 tile_load4(const __amdgpu_buffer_rsrc_t rsrc, const int row, const int stride, const int col, const int d) {
+    const unsigned at = (unsigned)(row * stride + col) * 4u;
+    if (VEC) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(col < d ? at : NOWHERE), 0, 0));
+    f32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        r[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)(col + e < d ? at + 4u * e : NOWHERE), 0, 0));
+    return r;
+}
+
+// Tiles of R rows x C columns in LDS as planes.
 //   Rows: [plane][row][C + 8]: a lane's eight columns are one 128-bit read, eight rows fall on distinct banks.
 //   Columns (the transposed tile): [plane][column][R], the rows of each 16 in the order 0-3, 8-11, 4-7, 12-15, so that the
 //   eight rows a lane needs against an accumulator's register order are one 128-bit read; 16-byte pieces of a column
@@ -126,83 +222,124 @@ __device__ __forceinline__ f32x16 mma6(const Frag &a, const Frag &b, f32x16 c) {
 template <int R, int C>
 struct Tile {
     static constexpr int ROWS_PLANE = R * (C + 8), COLS_PLANE = C * R;     // 16-bit elements
-    static constexpr int NROW = R * C / 1024;                              // float4 pieces per thread
-    static constexpr int QUADS = (R / 4) * (C / 4);                        // 4 x 4 pieces, at most one per thread
-    static_assert(R * C % 1024 == 0 && QUADS <= 256 && (R == 32 || R == 64) && C % 32 == 0, "tile");
+    static_assert((R == 32 || R == 64) && C % 32 == 0, "tile");
 
     __device__ static __forceinline__ int swap(const int col) {
         return R == 64 ? ((col >> 2) & 7) ^ ((col & 3) << 1) : ((col >> 1) ^ (col >> 3)) & 3;
-    }
-    // thread's piece i of the row form: row, column
-    __device__ static __forceinline__ int row_of(const int i) { return (threadIdx.x + 256 * i) / (C / 4); }
-    __device__ static __forceinline__ int col_of(const int i) { return (threadIdx.x + 256 * i) % (C / 4) * 4; }
-    __device__ static __forceinline__ void load_rows(f32x4 (&x)[NROW], const float *base, const long long stride, const int r0,
-                                                     const int rows, const int d, const bool vec) {
-#pragma unroll
-        for (int i = 0; i < NROW; ++i) {
-            const int r = r0 + row_of(i);
-            x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (r < rows) x[i] = load4(base + r * stride, col_of(i), d, vec);
-        }
-    }
-    __device__ static __forceinline__ void store_rows(u16 *t, const f32x4 (&x)[NROW]) {
-#pragma unroll
-        for (int i = 0; i < NROW; ++i) {
-            const Planes a = split2(x[i].x, x[i].y), b = split2(x[i].z, x[i].w);
-            u16 *p = t + row_of(i) * (C + 8) + col_of(i);
-            *reinterpret_cast<u32x2 *>(p) = u32x2{a.h, b.h};
-            *reinterpret_cast<u32x2 *>(p + ROWS_PLANE) = u32x2{a.m, b.m};
-            *reinterpret_cast<u32x2 *>(p + 2 * ROWS_PLANE) = u32x2{a.l, b.l};
-        }
-    }
-    // thread's 4 x 4 piece of the column form
-    __device__ static __forceinline__ int quad_row() { return threadIdx.x / (C / 4) * 4; }
-    __device__ static __forceinline__ int quad_col() { return threadIdx.x % (C / 4) * 4; }
-    __device__ static __forceinline__ bool has_quad() { return QUADS == 256 || threadIdx.x < QUADS; }
-    __device__ static __forceinline__ void load_quad(f32x4 (&x)[4], const float *base, const long long stride, const int r0,
-                                                     const int rows, const int d, const bool vec) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = r0 + quad_row() + i;
-            x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (has_quad() && r < rows) x[i] = load4(base + r * stride, quad_col(), d, vec);
-        }
-    }
-    __device__ static __forceinline__ void store_cols(u16 *t, const f32x4 (&x)[4]) {
-        if (!has_quad()) return;
-        const int kq = quad_row() >> 2;
-        const int piece = 2 * (kq >> 2) + (kq & 1), sub = 4 * ((kq >> 1) & 1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = quad_col() + j;
-            const Planes a = split2(x[0][j], x[1][j]), b = split2(x[2][j], x[3][j]);
-            u16 *p = t + col * R + ((piece ^ swap(col)) << 3) + sub;
-            *reinterpret_cast<u32x2 *>(p) = u32x2{a.h, b.h};
-            *reinterpret_cast<u32x2 *>(p + COLS_PLANE) = u32x2{a.m, b.m};
-            *reinterpret_cast<u32x2 *>(p + 2 * COLS_PLANE) = u32x2{a.l, b.l};
-        }
     }
     // operand of rows [32 sub, 32 sub + 32), columns [16 step, 16 step + 16): lane = row, eight columns
     __device__ static __forceinline__ Frag rows_frag(const u16 *t, const int sub, const int step) {
         const int lane = threadIdx.x & 63;
         const u16 *p = t + (32 * sub + (lane & 31)) * (C + 8) + 16 * step + 8 * (lane >> 5);
-        return Frag{*reinterpret_cast<const bf16x8 *>(p), *reinterpret_cast<const bf16x8 *>(p + ROWS_PLANE),
-                    *reinterpret_cast<const bf16x8 *>(p + 2 * ROWS_PLANE)};
+        return Frag{*reinterpret_cast<const f16x8 *>(p), *reinterpret_cast<const f16x8 *>(p + ROWS_PLANE)};
     }
     // operand of columns [32 part, 32 part + 32), rows [16 step, 16 step + 16): lane = column, eight rows in accumulator order
     __device__ static __forceinline__ Frag cols_frag(const u16 *t, const int part, const int step) {
         const int lane = threadIdx.x & 63, col = 32 * part + (lane & 31);
         const u16 *p = t + col * R + (((2 * step + (lane >> 5)) ^ swap(col)) << 3);
-        return Frag{*reinterpret_cast<const bf16x8 *>(p), *reinterpret_cast<const bf16x8 *>(p + COLS_PLANE),
-                    *reinterpret_cast<const bf16x8 *>(p + 2 * COLS_PLANE)};
+        return Frag{*reinterpret_cast<const f16x8 *>(p), *reinterpret_cast<const f16x8 *>(p + COLS_PLANE)};
     }
 };
 
+// Two R x C tiles (A, B) staged together by 256 threads: a thread loads 4 x 4 pieces, splits them and writes them in row form
+// and / or, exchanged pairwise, in column form.  A tile's pieces are a whole number of wavefronts, so which tile a piece
+// belongs to is uniform over a wavefront.
+template <int R, int C, bool VEC>
+struct Stage {
+    typedef Tile<R, C> T;
+    static constexpr int QUADS = (R / 4) * (C / 4), NP = (2 * QUADS + 255) / 256;
+    static_assert(QUADS % 64 == 0, "pieces");
+    f32x4 x[NP][4];
+
+    __device__ static __forceinline__ int piece(const int i) { return threadIdx.x + 256 * i; }
+    __device__ static __forceinline__ bool whole(const int i) { return 256 * i + 256 <= 2 * QUADS; }
+    __device__ static __forceinline__ bool has(const int i) { return whole(i) || __builtin_amdgcn_readfirstlane(piece(i)) < 2 * QUADS; }
+    __device__ static __forceinline__ bool second(const int i) { return __builtin_amdgcn_readfirstlane(piece(i)) >= QUADS; }
+    __device__ static __forceinline__ int row(const int i) { return (piece(i) - second(i) * QUADS) / (C / 4) * 4; }
+    __device__ static __forceinline__ int col(const int i) { return (piece(i) - second(i) * QUADS) % (C / 4) * 4; }
+
+    // rows [r0, r0 + R) of both tensors, of which those below `rows` are valid; rows [hide0, hide1) are taken as zeros
+    __device__ __forceinline__ void load(const float *a, const float *b, const int stride, const int r0, const int rows, const int d,
+                                         const int hide0 = 0, const int hide1 = 0) {
+        const __amdgpu_buffer_rsrc_t ra = tile_rows(a, stride, r0, rows, R, d), rb = tile_rows(b, stride, r0, rows, R, d);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (!has(i)) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = tile_load4<VEC>(second(i) ? rb : ra, row(i) + j, stride, col(i), d);
+        }
+        if (r0 < hide1 && r0 + R > hide0) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = r0 + row(i) + j;
+                    if (r >= hide0 && r < hide1) x[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+        }
+    }
+    // The largest value of either tile as far as this wavefront holds it, to most[wave] (both >= 0).
+    __device__ __forceinline__ void find_largest(f32x2 *most) const {
+        f32x2 m = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (!has(i)) continue;
+            const float v = wave_max_abs(largest(x[i]));
+            if (second(i)) m.y = fmaxf(m.y, v); else m.x = fmaxf(m.x, v);
+        }
+        if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+    }
+    // pa, pb: powers of two; f0, f1: factors of tile A's values, multiplied in one after the other (where SCALED)
+    template <bool ROWS_A, bool COLS_A, bool ROWS_B, bool COLS_B, bool SCALED>
+    __device__ __forceinline__ void store(u16 *rows_a, u16 *cols_a, u16 *rows_b, u16 *cols_b, const float pa, const float pb,
+                                          const float f0 = 1.0f, const float f1 = 1.0f) const {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (!has(i)) continue;
+            if (second(i)) put<ROWS_B, COLS_B, false>(i, rows_b, cols_b, pb, f0, f1);
+            else put<ROWS_A, COLS_A, SCALED>(i, rows_a, cols_a, pa, f0, f1);
+        }
+    }
+    template <bool ROWS, bool COLS, bool SCALED>
+    __device__ __forceinline__ void put(const int i, u16 *rows, u16 *cols, const float p2, const float f0, const float f1) const {
+        Planes w[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f32x4 v = x[i][j];
+            if (SCALED) v = (v * f0) * f1;
+            v *= p2;
+            w[j][0] = split2(v.x, v.y);
+            w[j][1] = split2(v.z, v.w);
+            if (ROWS) {
+                u16 *tr = rows + (row(i) + j) * (C + 8) + col(i);
+                *reinterpret_cast<u32x2 *>(tr) = u32x2{w[j][0].h, w[j][1].h};
+                *reinterpret_cast<u32x2 *>(tr + T::ROWS_PLANE) = u32x2{w[j][0].l, w[j][1].l};
+            }
+        }
+        if (COLS) {
+            const int kq = row(i) >> 2, at = 2 * (kq >> 2) + (kq & 1), sub = 4 * ((kq >> 1) & 1);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                u16 *p = cols + (col(i) + c) * R + ((at ^ T::swap(col(i) + c)) << 3) + sub;
+                // the low or high halves of two rows' words, side by side
+                const unsigned pick = c & 1 ? 0x07060302u : 0x05040100u;
+                auto turn = [&](const unsigned r0, const unsigned r1) { return __builtin_amdgcn_perm(r1, r0, pick); };
+                *reinterpret_cast<u32x2 *>(p) = u32x2{turn(w[0][c >> 1].h, w[1][c >> 1].h), turn(w[2][c >> 1].h, w[3][c >> 1].h)};
+                *reinterpret_cast<u32x2 *>(p + T::COLS_PLANE) = u32x2{turn(w[0][c >> 1].l, w[1][c >> 1].l), turn(w[2][c >> 1].l, w[3][c >> 1].l)};
+            }
+        }
+    }
+};
+// What find_largest left, over the workgroup: uniform.
+__device__ __forceinline__ f32x2 largest_of(const f32x2 *most) {
+    f32x2 m = most[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) m = f32x2{fmaxf(m.x, most[w].x), fmaxf(m.y, most[w].y)};
+    return f32x2{__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m.x))), __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m.y)))};
+}
+
 // Row of register r of a 32 x 32 accumulator in the lane's half of the wavefront (the column is lane % 32).
 __device__ __forceinline__ constexpr int acc_row(const int r) { return 8 * (r >> 2) + (r & 3); }
-
-__device__ __forceinline__ float max_halves(const float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
-__device__ __forceinline__ float sum_halves(const float v) { return v + __shfl_xor(v, 32, 64); }
 
 // The registers [8 step, 8 step + 8) of an accumulator as the other operand of a product that contracts over its rows.
 __device__ __forceinline__ Frag acc_frag(const f32x16 &s, const int step) {

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 4 : (DT <= 128 ? 2 : 1)) void s
     const int x0 = split * a.chunk, x1 = min(seen, x0 + a.chunk);
 
     const int col = c0 + min(ln, nc - 1), hq = hk * a.group + col / a.Lq, iq = col % a.Lq;
-    const long long p = a.w.last_key ? (long long)len - 1 : a.w.q_offset + iq;
+    const int p = a.w.last_key ? len - 1 : a.w.q_offset + iq;
     float qf[DT / 4];
     {
         const float *qp = q + b * a.lq.b + hq * a.lq.h + iq * a.lq.l;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 4 : (DT <= 128 ? 2 : 1)) void s
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int j = key_at(4 * quad + r);
-            if (!(x + 4 * quad + r < x1 && j <= p && (j > p - a.w.window || j < a.w.sinks))) s[r] = -INFINITY;
+            s[r] = ((x + 4 * quad + r < x1) & sees(a.w, p, j, len)) ? s[r] : -INFINITY;
         }
         const float tmax = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
         // the reference maximum, one per row and shared by its four lanes, moves only when a weight would pass 2^8
