@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
 
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;
-    Stage<32, DT, VEC> kv;
+    Stage<32, DT, VEC> kv(ks, g.d);
     if (at.tiles > 0) {
         kv.load(kp, vp, ks, at.key0(0), min(at.len, at.wp1 + 1), g.d, hide0, hide1);
         kv.find_largest(most);
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256, DT <= 64 ? 2 : 1) void sdpa_window_dkv_f32(con
     const int per_head = b0 < len && t1 > t0 ? t1 - t0 : 0;
     const int all = per_head * g.group, from = (int)((long long)all * chunk / kb.chunks[cl]), to = (int)((long long)all * (chunk + 1) / kb.chunks[cl]);
 
-    Stage<32, DT, VEC> qg;
+    Stage<32, DT, VEC> qg((int)g.lq.l, g.d);
     float sv = 0.f;
     auto load = [&](const int e) {
         const int h = hk * g.group + e / per_head, r0 = (t0 + e % per_head) * 32;

@@ -107,16 +107,25 @@ __device__ __forceinline__ float wave_max_abs(float v) {
                    r3 = __builtin_amdgcn_readlane(u, 48);
     return __uint_as_float(max(max(r0, r1), max(r2, r3)));
 }
+// max(m, |a|, |b|) without the quieting of signalling NaNs that fmaxf brings along (a NaN is passed over)
+__device__ __forceinline__ float max_abs(const float m, const float a, const float b) {
+    float r;
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(m), "v"(a), "v"(b));
+    return r;
+}
 template <int N>
-__device__ __forceinline__ float largest(const f32x4 (&x)[N]) {
+__device__ __forceinline__ float largest(const f32x4 (&x)[N], float m = 0.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max_abs(max_abs(m, x[i].x, x[i].y), x[i].z, x[i].w);
+    return m;
+}
+// Infinities do not set the scale of their neighbours: the largest finite value, for the rare case that `largest` met one.
+template <int N>
+__device__ __forceinline__ float largest_finite(const f32x4 (&x)[N]) {
     float m = 0.f;
+    asm volatile("" ::: "memory");                 // (not to be formed ahead of the question whether it is needed)
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = fmaxf(fmaxf(m, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-    if (__any(!(m < INFINITY))) {      // infinities do not set the scale of their neighbours
-        m = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) m = fmaxf(fmaxf(m, fmaxf(finite_abs(x[i].x), finite_abs(x[i].y))), fmaxf(finite_abs(x[i].z), finite_abs(x[i].w)));
-    }
+    for (int i = 0; i < N; ++i) m = fmaxf(fmaxf(m, fmaxf(finite_abs(x[i].x), finite_abs(x[i].y))), fmaxf(finite_abs(x[i].z), finite_abs(x[i].w)));
     return m;
 }
 
@@ -182,7 +191,9 @@ __device__ __forceinline__ int row_operand(Frag (&f)[DT / 16], const Load load, 
     for (int i = 0; i < DT / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[i][e] = (x[i][e] * f0) * f1;
-    const int a = scale_of(max_halves(largest(x)));
+    float top = max_halves(largest(x));
+    if (__any(top == INFINITY)) top = max_halves(largest_finite(x));
+    const int a = scale_of(top);
     const float p = pow2(a);
 #pragma unroll
     for (int s = 0; s < DT / 16; ++s) {
@@ -202,14 +213,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const float *base, c
     const int m = min(rows - r0, n);
     return __builtin_amdgcn_make_buffer_rsrc((void *)(base + (long long)r0 * stride), 0, m > 0 ? ((m - 1) * stride + d) * 4 : 0, 0x00020000);
 }
+// at: byte offset of the piece's first column, NOWHERE (or above) where the piece lies outside; left: columns from it to d
 template <bool VEC>
-__device__ __forceinline__ f32x4 tile_load4(const __amdgpu_buffer_rsrc_t rsrc, const int row, const int stride, const int col, const int d) {
-    const unsigned at = (unsigned)(row * stride + col) * 4u;
-    if (VEC) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(col < d ? at : NOWHERE), 0, 0));
+__device__ __forceinline__ f32x4 tile_load4(const __amdgpu_buffer_rsrc_t rsrc, const unsigned at, const int left) {
+    if (VEC) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at, 0, 0));
     f32x4 r;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        r[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)(col + e < d ? at + 4u * e : NOWHERE), 0, 0));
+        r[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)(e < left ? at + 4u * e : NOWHERE), 0, 0));
     return r;
 }
 
@@ -250,14 +261,29 @@ struct Stage {
     static constexpr int QUADS = (R / 4) * (C / 4), NP = (2 * QUADS + 255) / 256;
     static_assert(QUADS % 64 == 0, "pieces");
     f32x4 x[NP][4];
+    unsigned from[NP];       // byte offset of the thread's piece in its tensor's tile
+    int to_row[NP], to_col[NP];
 
     __device__ static __forceinline__ int piece(const int i) { return threadIdx.x + 256 * i; }
     __device__ static __forceinline__ bool whole(const int i) { return 256 * i + 256 <= 2 * QUADS; }
     __device__ static __forceinline__ bool has(const int i) { return whole(i) || __builtin_amdgcn_readfirstlane(piece(i)) < 2 * QUADS; }
-    __device__ static __forceinline__ bool second(const int i) { return __builtin_amdgcn_readfirstlane(piece(i)) >= QUADS; }
+    __device__ static __forceinline__ bool second(const int i) {
+        return QUADS % 256 == 0 ? 256 * i >= QUADS : __builtin_amdgcn_readfirstlane(piece(i)) >= QUADS;
+    }
     __device__ static __forceinline__ int row(const int i) { return (piece(i) - second(i) * QUADS) / (C / 4) * 4; }
     __device__ static __forceinline__ int col(const int i) { return (piece(i) - second(i) * QUADS) % (C / 4) * 4; }
 
+    __device__ __forceinline__ Stage(const int stride, const int d) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            from[i] = col(i) < d ? (unsigned)(row(i) * stride + col(i)) * 4u : NOWHERE;
+            to_row[i] = row(i) * (C + 8) + col(i);
+            // column form: four rows of a column are one 8-byte write; the piece's exchange takes in the column's low bits by
+            // an exclusive or with a constant
+            const int kq = row(i) >> 2, at = 2 * (kq >> 2) + (kq & 1), sub = 4 * ((kq >> 1) & 1);
+            to_col[i] = col(i) * R + ((at ^ T::swap(col(i))) << 3) + sub;
+        }
+    }
     // rows [r0, r0 + R) of both tensors, of which those below `rows` are valid; rows [hide0, hide1) are taken as zeros
     __device__ __forceinline__ void load(const float *a, const float *b, const int stride, const int r0, const int rows, const int d,
                                          const int hide0 = 0, const int hide1 = 0) {
@@ -266,9 +292,10 @@ struct Stage {
         for (int i = 0; i < NP; ++i) {
             if (!has(i)) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][j] = tile_load4<VEC>(second(i) ? rb : ra, row(i) + j, stride, col(i), d);
+            for (int j = 0; j < 4; ++j) x[i][j] = tile_load4<VEC>(second(i) ? rb : ra, from[i] + 4u * j * stride, VEC ? 0 : d - col(i));
         }
         if (r0 < hide1 && r0 + R > hide0) {
+            asm volatile("" ::: "memory");
 #pragma unroll
             for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -280,12 +307,21 @@ struct Stage {
     }
     // The largest value of either tile as far as this wavefront holds it, to most[wave] (both >= 0).
     __device__ __forceinline__ void find_largest(f32x2 *most) const {
-        f32x2 m = {0.f, 0.f};
+        float v[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             if (!has(i)) continue;
-            const float v = wave_max_abs(largest(x[i]));
-            if (second(i)) m.y = fmaxf(m.y, v); else m.x = fmaxf(m.x, v);
+            if (second(i)) v[1] = largest(x[i], v[1]); else v[0] = largest(x[i], v[0]);
+        }
+        f32x2 m = {wave_max_abs(v[0]), wave_max_abs(v[1])};
+        if (m.x == INFINITY || m.y == INFINITY) {
+            v[0] = v[1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                if (!has(i)) continue;
+                if (second(i)) v[1] = fmaxf(v[1], largest_finite(x[i])); else v[0] = fmaxf(v[0], largest_finite(x[i]));
+            }
+            m = f32x2{wave_max_abs(v[0]), wave_max_abs(v[1])};
         }
         if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
     }
@@ -311,16 +347,15 @@ struct Stage {
             w[j][0] = split2(v.x, v.y);
             w[j][1] = split2(v.z, v.w);
             if (ROWS) {
-                u16 *tr = rows + (row(i) + j) * (C + 8) + col(i);
+                u16 *tr = rows + to_row[i] + j * (C + 8);
                 *reinterpret_cast<u32x2 *>(tr) = u32x2{w[j][0].h, w[j][1].h};
                 *reinterpret_cast<u32x2 *>(tr + T::ROWS_PLANE) = u32x2{w[j][0].l, w[j][1].l};
             }
         }
         if (COLS) {
-            const int kq = row(i) >> 2, at = 2 * (kq >> 2) + (kq & 1), sub = 4 * ((kq >> 1) & 1);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                u16 *p = cols + (col(i) + c) * R + ((at ^ T::swap(col(i) + c)) << 3) + sub;
+                u16 *p = cols + (to_col[i] ^ (T::swap(c) << 3)) + c * R;
                 // the low or high halves of two rows' words, side by side
                 const unsigned pick = c & 1 ? 0x07060302u : 0x05040100u;
                 auto turn = [&](const unsigned r0, const unsigned r1) { return __builtin_amdgcn_perm(r1, r0, pick); };
