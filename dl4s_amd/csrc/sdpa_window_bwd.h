@@ -22,15 +22,32 @@ namespace {
 struct ColumnScale {
     int c = 0;
     bool fresh = true;
+    // The same for weights, which are at most 2^13: a column takes a power only where its first largest is below 2^-3.
+    __device__ __forceinline__ bool fit_tiny(f32x16 &w, float &factor, float &acc_factor) {
+        float m = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, w[r]);
+        m = max_halves(m);
+        const bool move = (c != 0 && m > 32768.0f) || (fresh && m > 0.f && m < 0.125f);
+        fresh = fresh && !(m > 0.f);
+        if (!__any(move)) return false;
+        // the largest to 2^8, with no power below zero
+        const int shift = !move ? 0 : max(min(135 - (int)(__float_as_uint(m) >> 23), 126), -c);
+        c += shift;
+        acc_factor = pow2(shift);
+        factor *= acc_factor;
+        w *= acc_factor;
+        return true;
+    }
     // ds: this tile's values under the present power.  Returns whether any lane's power moved; acc_factor is then the lane's
     // factor for what it has accumulated.
     __device__ __forceinline__ bool fit(f32x16 &ds, float &factor, float &acc_factor) {
         float m = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(ds[r]));
+        if (!__any(m > 32768.0f || (fresh && m > 0.f))) return false;
         m = max_halves(m);
         const bool move = m > 32768.0f || (fresh && m > 0.f);
-        if (!__any(move)) return false;
         const int shift = move ? min(max(135 - (int)(__float_as_uint(m) >> 23), -126), 126) : 0;
         fresh = fresh && !(m > 0.f);
         c += shift;
@@ -50,7 +67,7 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
     typedef Tile<32, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
     u16 *Ks = window_lds, *Vs = Ks + 2 * T::ROWS_PLANE, *Kc = Vs + 2 * T::ROWS_PLANE;
-    __shared__ f32x2 most[4];
+    __shared__ __align__(16) int powers[2][4];             // [K, V]
 
     const int unit = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
     if (unit >= g.units) return;
@@ -60,21 +77,19 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;
     Stage<32, DT, VEC> kv(ks, g.d);
-    if (at.tiles > 0) {
-        kv.load(kp, vp, ks, at.key0(0), min(at.len, at.wp1 + 1), g.d, hide0, hide1);
-        kv.find_largest(most);
-    }
+    auto load = [&](const int i) { kv.load(kp, vp, ks, at.key0(i), min(at.len, at.wp1 + 1), g.d, hide0, hide1); };
+    if (at.tiles > 0) load(0);
 
     const long long el = at.b * g.lq.b + at.h * g.lq.h + at.qc * g.lq.l, row = ((long long)at.b * g.H + at.h) * g.Lq + at.qc;
     Frag qf[DT / 16], gf[DT / 16];
-    const int aq = row_operand<DT>(qf, [&](const int c) { return load4(q + el, c, g.d, VEC); }, g.rT, LOG2E);
+    const float unq = pow2(-row_operand<DT>(qf, [&](const int c) { return load4(q + el, c, g.d, VEC); }, g.rT, LOG2E));
     float del = 0.f;
-    const int ag = row_operand<DT>(gf, [&](const int c) {
+    const float ung = pow2(-row_operand<DT>(gf, [&](const int c) {
         const f32x4 x = load4(dout + el, c, g.d, VEC), o = load4(out + el, c, g.d, VEC);
 #pragma unroll
         for (int e = 0; e < 4; ++e) del += x[e] * o[e];
         return x;
-    }, 1.0f, 1.0f);
+    }, 1.0f, 1.0f));
     del = sum_halves(del);
     const float m = stats[2 * row], inv = stats[2 * row + 1];
     if (half == 0 && at.qi < g.Lq) delta[row] = del;
@@ -88,56 +103,59 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     ColumnScale scale;
     float factor = inv;                                    // dS as an operand = 2^(s - m) (dP - delta) factor
-    int ak = 126;
+    int nk = -63;                                          // acc is in units of 2^nk
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
-        const f32x2 top = largest_of(most);
-        const int ak_new = min(ak, scale_of(top.x)), av = scale_of(top.y);
-        if (ak_new != ak) {
-            const float f = pow2(max(ak_new - ak, -126));
-#pragma unroll
-            for (int t = 0; t < DT / 32; ++t) acc[t] *= f;
-            ak = ak_new;
-        }
-        kv.template store<true, true, true, false, false>(Ks, Kc, Vs, nullptr, pow2(ak), pow2(av));
+        kv.template store<true, true, true, false, false>(Ks, Kc, Vs, nullptr, &powers[0][0]);
         __syncthreads();
-        if (i + 1 < at.tiles) kv.load(kp, vp, ks, at.key0(i + 1), min(at.len, at.wp1 + 1), g.d, hide0, hide1);
+        if (i + 1 < at.tiles) load(i + 1);
         const int k0 = at.key0(i);
-        if (!(idle || tile_hidden(g.w, p0, p1, k0, at.len))) {
-            f32x16 s, dp;
+        if (idle || tile_hidden(g.w, p0, p1, k0, at.len)) continue;
+        f32x16 s, dp;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
-            for (int st = 0; st < DT / 16; ++st) {
-                s = mma3(T::rows_frag(Ks, 0, st), qf[st], s);
-                dp = mma3(T::rows_frag(Vs, 0, st), gf[st], dp);
-            }
-            if (!tile_open(g.w, p0, p1, k0, at.len)) {
+        for (int st = 0; st < DT / 16; ++st)
+            mma3x2(s, T::rows_frag(Ks, 0, st), qf[st], dp, T::rows_frag(Vs, 0, st), gf[st]);
+        const Powers kn(powers[0]);
+        const i32x4 vn = *reinterpret_cast<const i32x4 *>(powers[1]);
+        settle(s, dp);
+        const float del_f = del * factor;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = sees(g.w, p, k0 + acc_row(r) + 4 * half, at.len) ? s[r] : -INFINITY;
-            }
-            const float f = pow2(max(-(aq + ak), -126)), fp = pow2(-(ag + av));
+        for (int x = 0; x < 4; ++x) {
+            const float f = __builtin_ldexpf(unq, kn.n[x]), fp = __builtin_ldexpf(ung, vn[x]) * factor;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                s[r] = (exp2_fast(__builtin_fmaf(s[r], f, -m)) * __builtin_fmaf(dp[r], fp, -del)) * factor;
-            float shrink;
-            if (scale.fit(s, factor, shrink)) {
-#pragma unroll
-                for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
-            }
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                const Frag df = acc_frag(s, st);
-#pragma unroll
-                for (int t = 0; t < DT / 32; ++t) acc[t] = mma3(T::cols_frag(Kc, t, st), df, acc[t]);
-            }
+            for (int r = 4 * x; r < 4 * x + 4; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], f, -m)) * __builtin_fmaf(dp[r], fp, -del_f);
         }
-        if (i + 1 < at.tiles) kv.find_largest(most);
+        if (!tile_open(g.w, p0, p1, k0, at.len)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = sees(g.w, p, k0 + acc_row(r) + 4 * half, at.len) ? s[r] : 0.f;
+        }
+        if (kn.lo != nk || kn.hi != nk) {
+            const float unit = to_one_unit(kn, nk, s);
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
+        }
+        float shrink;
+        if (scale.fit(s, factor, shrink)) {
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            const Frag df = acc_frag(s, st);
+            Frag kc[DT / 32];
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) kc[t] = T::cols_frag(Kc, t, st);
+            mma3(acc, kc, df);
+        }
     }
 
+#pragma unroll
+    for (int t = 0; t < DT / 32; ++t) settle(acc[t]);
     if (at.qi >= g.Lq) return;
-    const float f0 = pow2(-scale.c), f1 = pow2(-ak);
+    const float f0 = pow2(-scale.c), f1 = pow2(nk);
     const bool empty = inv == 0.f;                         // saw no key: no gradient, whatever stands in its rows
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
@@ -178,8 +196,8 @@ __global__ __launch_bounds__(256, DT <= 64 ? 2 : 1) void sdpa_window_dkv_f32(con
     typedef Tile<32, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
     u16 *Qs = window_lds, *Gs = Qs + 2 * T::ROWS_PLANE, *Qc = Gs + 2 * T::ROWS_PLANE, *Gc = Qc + 2 * T::COLS_PLANE;
-    __shared__ __align__(16) float rowv[96];               // [3][32]: m, 1 / l, delta of the tile's queries
-    __shared__ f32x2 most[4];
+    __shared__ __align__(16) float rowv[96];               // [3][32]: m, 2^13 / l, delta of the tile's queries
+    __shared__ __align__(16) int powers[2][4];             // [Q, dO]
 
     int id = blockIdx.x, cl = 0;
     if (id >= 8 * kb.per_xcd[0]) { id -= 8 * kb.per_xcd[0]; cl = 1; }
@@ -209,104 +227,108 @@ __global__ __launch_bounds__(256, DT <= 64 ? 2 : 1) void sdpa_window_dkv_f32(con
             const int which = threadIdx.x >> 5, r = r0 + (threadIdx.x & 31);
             const long long row = ((long long)b * g.H + h) * g.Lq + r;
             sv = r < rows ? (which == 2 ? delta[row] : stats[2 * row + which]) : 0.f;
+            if (which == 1) sv *= 8192.0f;
         }
     };
-    if (from < to) {
-        load(from);
-        qg.find_largest(most);
-    }
+    if (from < to) load(from);
 
     Frag kf[DT / 16], vf[DT / 16];
     const long long el = b * g.lk.b + hk * g.lk.h + key * g.lk.l;
     auto key_row = [&](const float *x) {
         return [=](const int c) { return key < len ? load4(x + el, c, g.d, VEC) : f32x4{0.f, 0.f, 0.f, 0.f}; };
     };
-    const int ak = row_operand<DT>(kf, key_row(k), 1.0f, 1.0f), av = row_operand<DT>(vf, key_row(v), 1.0f, 1.0f);
+    const float unk = pow2(-row_operand<DT>(kf, key_row(k), 1.0f, 1.0f)), unv = pow2(-row_operand<DT>(vf, key_row(v), 1.0f, 1.0f));
 
     f32x16 dka[DT / 32], dva[DT / 32];
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) { dka[t][r] = 0.f; dva[t][r] = 0.f; }
+    // The operands are 2^13 w, times a power of two where a column's weights are all tiny, and w (dP - delta) factor.
     ColumnScale wscale, scale;
-    float wfactor = 1.0f, factor = 1.0f;                   // the operands are w wfactor and w (dP - delta) factor
-    int aq = 126, ag = 126;
-    const float q_size = fabsf(g.rT) * LOG2E;
+    float wfactor = 1.0f, factor = 1.0f / 8192;
+    bool plain = false;                                    // every column has met a weight that needs no power
+    int nq = -63, ng = -63;                                // dka, dva are in units of 2^nq, 2^ng
 
     for (int e = from; e < to; ++e) {
         __syncthreads();
-        const f32x2 top = largest_of(most);
-        const int aq_new = min(aq, scale_of(top.x * q_size)), ag_new = min(ag, scale_of(top.y));
-        if (aq_new != aq || ag_new != ag) {
-            const float fq = pow2(max(aq_new - aq, -126)), fg = pow2(max(ag_new - ag, -126));
-#pragma unroll
-            for (int t = 0; t < DT / 32; ++t) { dka[t] *= fq; dva[t] *= fg; }
-            aq = aq_new;
-            ag = ag_new;
-        }
-        qg.template store<true, true, true, true, true>(Qs, Qc, Gs, Gc, pow2(aq), pow2(ag), g.rT, LOG2E);
+        qg.template store<true, true, true, true, true>(Qs, Qc, Gs, Gc, &powers[0][0], g.rT, LOG2E);
         if (threadIdx.x < 96) rowv[threadIdx.x] = sv;
         __syncthreads();
         if (e + 1 < to) load(e + 1);
         const int q0 = (t0 + e % per_head) * 32;
         const int p0 = g.w.q_offset + q0, p1 = g.w.q_offset + min(q0 + 31, g.Lq - 1);
-        if (!tile_hidden(g.w, p0, p1, k0, len)) {
-            f32x16 s, dp;
+        if (tile_hidden(g.w, p0, p1, k0, len)) continue;
+        f32x16 s, dp;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
-            for (int st = 0; st < DT / 16; ++st) {
-                s = mma3(T::rows_frag(Qs, 0, st), kf[st], s);
-                dp = mma3(T::rows_frag(Gs, 0, st), vf[st], dp);
+        for (int st = 0; st < DT / 16; ++st)
+            mma3x2(s, T::rows_frag(Qs, 0, st), kf[st], dp, T::rows_frag(Gs, 0, st), vf[st]);
+        const Powers qn(powers[0]), gn(powers[1]);
+        settle(s, dp);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const f32x4 m = *reinterpret_cast<const f32x4 *>(rowv + 8 * x + 4 * half), inv = *reinterpret_cast<const f32x4 *>(rowv + 32 + 8 * x + 4 * half),
+                        del = *reinterpret_cast<const f32x4 *>(rowv + 64 + 8 * x + 4 * half);
+            const float f = __builtin_ldexpf(unk, qn.n[x]), fp = __builtin_ldexpf(unv, gn.n[x]);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int r = 4 * x + y;
+                s[r] = exp2_fast(__builtin_fmaf(s[r], f, -m[y])) * inv[y];
+                dp[r] = (s[r] * __builtin_fmaf(dp[r], fp, -del[y])) * factor;
             }
-            const bool open = tile_open(g.w, p0, p1, k0, len) && q0 + 32 <= g.Lq;
-            const float f = pow2(max(-(aq + ak), -126)), fp = pow2(-(ag + av));
+        }
+        if (!(tile_open(g.w, p0, p1, k0, len) && q0 + 32 <= g.Lq)) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const f32x4 m = *reinterpret_cast<const f32x4 *>(rowv + 8 * x + 4 * half), inv = *reinterpret_cast<const f32x4 *>(rowv + 32 + 8 * x + 4 * half),
-                            del = *reinterpret_cast<const f32x4 *>(rowv + 64 + 8 * x + 4 * half);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int r = 4 * x + y, i = q0 + 8 * x + 4 * half + y;
-                    const float w = exp2_fast(__builtin_fmaf(s[r], f, -m[y])) * inv[y];
-                    s[r] = w * wfactor;
-                    dp[r] = (w * __builtin_fmaf(dp[r], fp, -del[y])) * factor;
-                    if (!open) {
-                        const bool see = (i < g.Lq) & sees(g.w, g.w.q_offset + i, key, len);
-                        s[r] = see ? s[r] : 0.f;
-                        dp[r] = see ? dp[r] : 0.f;
-                    }
-                }
+            for (int r = 0; r < 16; ++r) {
+                const int i = q0 + acc_row(r) + 4 * half;
+                const bool see = (i < g.Lq) & sees(g.w, g.w.q_offset + i, key, len);
+                s[r] = see ? s[r] : 0.f;
+                dp[r] = see ? dp[r] : 0.f;
             }
+        }
+        if (!plain) {
+            s *= wfactor;
             float shrink;
-            if (wscale.fit(s, wfactor, shrink)) {
+            if (wscale.fit_tiny(s, wfactor, shrink)) {
 #pragma unroll
                 for (int t = 0; t < DT / 32; ++t) dva[t] *= shrink;
             }
-            if (scale.fit(dp, factor, shrink)) {
-#pragma unroll
-                for (int t = 0; t < DT / 32; ++t) dka[t] *= shrink;
-            }
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                const Frag wf = acc_frag(s, st), df = acc_frag(dp, st);
-#pragma unroll
-                for (int t = 0; t < DT / 32; ++t) {
-                    dva[t] = mma3(T::cols_frag(Gc, t, st), wf, dva[t]);
-                    dka[t] = mma3(T::cols_frag(Qc, t, st), df, dka[t]);
-                }
-            }
+            plain = !__any(wscale.fresh || wscale.c != 0);
         }
-        if (e + 1 < to) qg.find_largest(most);
+        if (qn.lo != nq || qn.hi != nq) {
+            const float unit = to_one_unit(qn, nq, dp);
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) dka[t] *= unit;
+        }
+        if (gn.lo != ng || gn.hi != ng) {
+            const float unit = to_one_unit(gn, ng, s);
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) dva[t] *= unit;
+        }
+        float shrink;
+        if (scale.fit(dp, factor, shrink)) {
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) dka[t] *= shrink;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            const Frag wf = acc_frag(s, st), df = acc_frag(dp, st);
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) mma3x2(dva[t], T::cols_frag(Gc, t, st), wf, dka[t], T::cols_frag(Qc, t, st), df);
+        }
     }
 
+#pragma unroll
+    for (int t = 0; t < DT / 32; ++t) settle(dka[t], dva[t]);
     if (key >= g.Lk) return;
     // q was staged as q rT log2(e): dk = rT sum dS q = ln(2) of what was summed
     constexpr float LN2 = 0.69314718055994530942f;
     const bool whole = kb.chunks[cl] == 1;
     float *part = whole ? nullptr : partial_sums(kb, pair, block, chunk, g.d) + (wave * 32 + ln) * (long long)g.d;
     float *ok = whole ? dk + el : part, *ov = whole ? dv + el : part + 128ll * g.d;
-    const float k0f = pow2(-scale.c), k1f = pow2(-aq), vf0 = pow2(-wscale.c), vf1 = pow2(-ag);
+    const float k0f = pow2(-scale.c), k1f = pow2(nq), vf0 = pow2(-13 - wscale.c), vf1 = pow2(ng);
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll

@@ -86,10 +86,16 @@ __device__ __forceinline__ void store4(float *row, const int col, const int d, c
 
 // ---- powers of two
 __device__ __forceinline__ float pow2(const int a) { return __builtin_ldexpf(1.0f, a); }
-// The power that puts m (>= 0, finite) into [2^14, 2^15); tiny m stop at 2^125, which is as good.
+// The power that puts m (>= 0, finite) into [2^14, 2^15).  m below 2^-49 stays below: two such powers and the scores they
+// belong to keep within the range of fp32, and what is lost are bits below 2^-73.
 __device__ __forceinline__ int scale_of(const float m) {
     const int e = (int)(__float_as_uint(m) >> 23);
-    return 141 - min(max(e, 16), 254);
+    return 141 - min(max(e, 78), 254);
+}
+// The same in steps of 2^8 ([2^7, 2^15)): neighbouring rows of like size then mostly have the same power.
+__device__ __forceinline__ int coarse_scale_of(const float m) {
+    const int e = (int)(__float_as_uint(m) >> 23);
+    return 141 - min(((max(e, 78) + 3) & ~7) + 4, 256);
 }
 __device__ __forceinline__ float finite_abs(const float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
 template <int CTRL>
@@ -133,25 +139,25 @@ __device__ __forceinline__ float largest_finite(const f32x4 (&x)[N]) {
 struct Planes {
     unsigned h, l;
 };
-// x minus the low / high half of h, one instruction each
-__device__ __forceinline__ float minus_low(const float x, const unsigned h) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(x), "v"(h));
-    return r;
-}
-__device__ __forceinline__ float minus_high(const float x, const unsigned h) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(x), "v"(h));
-    return r;
-}
+// v_fma_mixlo_f16 / v_fma_mixhi_f16 round an fp32 multiply-add to fp16 into the low / high half of their result.  A half that was
+// moved up may be read one wait state later at the earliest; the compiler does not look into the statement, so it ends
+// with that state.
 __device__ __forceinline__ unsigned round2(const float a, const float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
-__device__ __forceinline__ Planes split2(const float a, const float b) {
-    Planes p;
-    p.h = round2(a, b);
-    p.l = round2(minus_low(a, p.h), minus_high(b, p.h));
-    return p;
+// The planes of four values times a power of two s.
+__device__ __forceinline__ void split4(const f32x4 v, const float s, Planes &p, Planes &q) {
+    asm("v_fma_mixlo_f16 %0, %4, %8, 0\n\t"
+        "v_fma_mixhi_f16 %0, %5, %8, 0\n\t"
+        "v_fma_mixlo_f16 %2, %6, %8, 0\n\t"
+        "v_fma_mixhi_f16 %2, %7, %8, 0\n\t"
+        "v_fma_mixlo_f16 %1, %4, %8, -%0 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %1, %5, %8, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixlo_f16 %3, %6, %8, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %3, %7, %8, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "s_nop 0"
+        : "=&v"(p.h), "=&v"(p.l), "=&v"(q.h), "=&v"(q.l)
+        : "v"(v.x), "v"(v.y), "v"(v.z), "v"(v.w), "v"(s));
 }
 
 // One lane's share of an operand of a 32 x 32 x 16 step: eight values along the contraction, as planes.
@@ -161,10 +167,20 @@ struct Frag {
 __device__ __forceinline__ Frag split8(const float (&x)[8]) {
     u32x4 h, l;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const Planes p = split2(x[2 * i], x[2 * i + 1]);
-        h[i] = p.h; l[i] = p.l;
-    }
+    for (int i = 0; i < 4; ++i) h[i] = round2(x[2 * i], x[2 * i + 1]);
+    unsigned l0, l1, l2, l3;
+    asm("v_fma_mixlo_f16 %0, %4, 1.0, -%12 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixlo_f16 %1, %6, 1.0, -%13 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixlo_f16 %2, %8, 1.0, -%14 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixlo_f16 %3, %10, 1.0, -%15 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %0, %5, 1.0, -%12 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %1, %7, 1.0, -%13 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %2, %9, 1.0, -%14 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %3, %11, 1.0, -%15 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "s_nop 0"
+        : "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3)
+        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]), "v"(h.x), "v"(h.y), "v"(h.z), "v"(h.w));
+    l = u32x4{l0, l1, l2, l3};
     return Frag{__builtin_bit_cast(f16x8, h), __builtin_bit_cast(f16x8, l)};
 }
 __device__ __forceinline__ f32x16 mma3(const Frag &a, const Frag &b, f32x16 c) {
@@ -172,9 +188,40 @@ __device__ __forceinline__ f32x16 mma3(const Frag &a, const Frag &b, f32x16 c) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.l, c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
 }
+// The three instructions of a product go to an accumulator one after the other; the accumulators c[0 .. N) take turns, because
+// an instruction that adds to the accumulator of the one before it waits for it.
+template <int N>
+__device__ __forceinline__ void mma3(f32x16 (&c)[N], const Frag (&a)[N], const Frag &b) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) c[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n].l, b.h, c[n], 0, 0, 0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) c[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n].h, b.l, c[n], 0, 0, 0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) c[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n].h, b.h, c[n], 0, 0, 0);
+}
+// Two products at once, each with operands of its own.
+__device__ __forceinline__ void mma3x2(f32x16 &c0, const Frag &a0, const Frag &b0, f32x16 &c1, const Frag &a1, const Frag &b1) {
+    c0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0.l, b0.h, c0, 0, 0, 0);
+    c1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1.l, b1.h, c1, 0, 0, 0);
+    c0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0.h, b0.l, c0, 0, 0, 0);
+    c1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1.h, b1.l, c1, 0, 0, 0);
+    c0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a0.h, b0.h, c0, 0, 0, 0);
+    c1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a1.h, b1.h, c1, 0, 0, 0);
+}
 
-__device__ __forceinline__ float max_halves(const float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
-__device__ __forceinline__ float sum_halves(const float v) { return v + __shfl_xor(v, 32, 64); }
+// The vector ALU may read an accumulator 12 wait states after the last matrix instruction that wrote it.  The compiler puts
+// them in, but not on a path that branches right behind the instructions (its assembly had one state there, and wrong
+// sums): results that a branch follows are waited for explicitly.
+__device__ __forceinline__ void settle(f32x16 &a) { asm volatile("s_nop 11" : "+v"(a)); }
+__device__ __forceinline__ void settle(f32x16 &a, f32x16 &b) { asm volatile("s_nop 11" : "+v"(a), "+v"(b)); }
+
+// With the value of lane ^ 32: both lanes end up with the same.
+__device__ __forceinline__ f32x2 both_halves(const float v) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f32x2{__uint_as_float(r.x), __uint_as_float(r.y)};
+}
+__device__ __forceinline__ float max_halves(const float v) { const f32x2 r = both_halves(v); return fmaxf(r.x, r.y); }
+__device__ __forceinline__ float sum_halves(const float v) { const f32x2 r = both_halves(v); return r.x + r.y; }
 
 // A row of up to DT columns, one row per lane of a half wavefront (lane and lane ^ 32 share it), as the operand whose
 // contraction runs along the row; f0 and f1 are multiplied in one after the other.  Returns the row's power of two.
@@ -197,10 +244,10 @@ __device__ __forceinline__ int row_operand(Frag (&f)[DT / 16], const Load load, 
     const float p = pow2(a);
 #pragma unroll
     for (int s = 0; s < DT / 16; ++s) {
-        float z[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { z[e] = x[2 * s][e] * p; z[4 + e] = x[2 * s + 1][e] * p; }
-        f[s] = split8(z);
+        Planes w[4];
+        split4(x[2 * s], p, w[0], w[1]);
+        split4(x[2 * s + 1], p, w[2], w[3]);
+        f[s] = Frag{__builtin_bit_cast(f16x8, (u32x4){w[0].h, w[1].h, w[2].h, w[3].h}), __builtin_bit_cast(f16x8, (u32x4){w[0].l, w[1].l, w[2].l, w[3].l})};
     }
     return a;
 }
@@ -253,25 +300,28 @@ struct Tile {
 };
 
 // Two R x C tiles (A, B) staged together by 256 threads: a thread loads 4 x 4 pieces, splits them and writes them in row form
-// and / or, exchanged pairwise, in column form.  A tile's pieces are a whole number of wavefronts, so which tile a piece
-// belongs to is uniform over a wavefront.
+// and / or, exchanged pairwise, in column form.  The pieces that a wavefront handles at a time are whole rows of one tile
+// (C is rounded up to a power of two for that), so it finds their largest value and their power of two by itself; the
+// powers go to LDS with the tile, one for every eight rows.
 template <int R, int C, bool VEC>
 struct Stage {
     typedef Tile<R, C> T;
-    static constexpr int QUADS = (R / 4) * (C / 4), NP = (2 * QUADS + 255) / 256;
-    static_assert(QUADS % 64 == 0, "pieces");
+    static constexpr int GROUPS = (C <= 32 ? 32 : (C <= 64 ? 64 : 128)) / 4;      // of four columns
+    static constexpr int QUADS = (R / 4) * GROUPS, NP = (2 * QUADS + 255) / 256, WAVE_ROWS = 256 / GROUPS;
+    static_assert(QUADS % 64 == 0 && WAVE_ROWS >= 8, "pieces");
     f32x4 x[NP][4];
     unsigned from[NP];       // byte offset of the thread's piece in its tensor's tile
     int to_row[NP], to_col[NP];
+    int run[2] = {63, 63};   // smallest power so far of the rows this wavefront stages of either tile
 
     __device__ static __forceinline__ int piece(const int i) { return threadIdx.x + 256 * i; }
-    __device__ static __forceinline__ bool whole(const int i) { return 256 * i + 256 <= 2 * QUADS; }
-    __device__ static __forceinline__ bool has(const int i) { return whole(i) || __builtin_amdgcn_readfirstlane(piece(i)) < 2 * QUADS; }
+    __device__ static __forceinline__ bool has(const int i) { return 256 * i + 256 <= 2 * QUADS || __builtin_amdgcn_readfirstlane(piece(i)) < 2 * QUADS; }
     __device__ static __forceinline__ bool second(const int i) {
         return QUADS % 256 == 0 ? 256 * i >= QUADS : __builtin_amdgcn_readfirstlane(piece(i)) >= QUADS;
     }
-    __device__ static __forceinline__ int row(const int i) { return (piece(i) - second(i) * QUADS) / (C / 4) * 4; }
-    __device__ static __forceinline__ int col(const int i) { return (piece(i) - second(i) * QUADS) % (C / 4) * 4; }
+    __device__ static __forceinline__ int row(const int i) { return (piece(i) - second(i) * QUADS) / GROUPS * 4; }
+    __device__ static __forceinline__ int col(const int i) { return piece(i) % GROUPS * 4; }
+    __device__ static __forceinline__ bool inside(const int i) { return C == 4 * GROUPS || col(i) < C; }
 
     __device__ __forceinline__ Stage(const int stride, const int d) {
 #pragma unroll
@@ -288,64 +338,50 @@ struct Stage {
     __device__ __forceinline__ void load(const float *a, const float *b, const int stride, const int r0, const int rows, const int d,
                                          const int hide0 = 0, const int hide1 = 0) {
         const __amdgpu_buffer_rsrc_t ra = tile_rows(a, stride, r0, rows, R, d), rb = tile_rows(b, stride, r0, rows, R, d);
+        const bool cut = r0 < hide1 && r0 + R > hide0;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             if (!has(i)) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][j] = tile_load4<VEC>(second(i) ? rb : ra, from[i] + 4u * j * stride, VEC ? 0 : d - col(i));
-        }
-        if (r0 < hide1 && r0 + R > hide0) {
-            asm volatile("" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
+            unsigned at[4] = {from[i], from[i] + 4u * stride, from[i] + 8u * stride, from[i] + 12u * stride};
+            if (__builtin_expect(cut, 0)) {
+                asm volatile("" : "+v"(at[0]), "+v"(at[1]), "+v"(at[2]), "+v"(at[3]));     // (keeps this a branch)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = r0 + row(i) + j;
-                    if (r >= hide0 && r < hide1) x[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (r >= hide0 && r < hide1) at[j] = NOWHERE;
                 }
-        }
-    }
-    // The largest value of either tile as far as this wavefront holds it, to most[wave] (both >= 0).
-    __device__ __forceinline__ void find_largest(f32x2 *most) const {
-        float v[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            if (!has(i)) continue;
-            if (second(i)) v[1] = largest(x[i], v[1]); else v[0] = largest(x[i], v[0]);
-        }
-        f32x2 m = {wave_max_abs(v[0]), wave_max_abs(v[1])};
-        if (m.x == INFINITY || m.y == INFINITY) {
-            v[0] = v[1] = 0.f;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                if (!has(i)) continue;
-                if (second(i)) v[1] = fmaxf(v[1], largest_finite(x[i])); else v[0] = fmaxf(v[0], largest_finite(x[i]));
             }
-            m = f32x2{wave_max_abs(v[0]), wave_max_abs(v[1])};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = tile_load4<VEC>(second(i) ? rb : ra, at[j], VEC ? 0 : d - col(i));
         }
-        if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
     }
-    // pa, pb: powers of two; f0, f1: factors of tile A's values, multiplied in one after the other (where SCALED)
+    // f0, f1: factors of tile A's values, multiplied in one after the other (where SCALED).  powers: [A, B][R / 8], negated.
     template <bool ROWS_A, bool COLS_A, bool ROWS_B, bool COLS_B, bool SCALED>
-    __device__ __forceinline__ void store(u16 *rows_a, u16 *cols_a, u16 *rows_b, u16 *cols_b, const float pa, const float pb,
-                                          const float f0 = 1.0f, const float f1 = 1.0f) const {
+    __device__ __forceinline__ void store(u16 *rows_a, u16 *cols_a, u16 *rows_b, u16 *cols_b, int *powers, const float f0 = 1.0f,
+                                          const float f1 = 1.0f) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             if (!has(i)) continue;
-            if (second(i)) put<ROWS_B, COLS_B, false>(i, rows_b, cols_b, pb, f0, f1);
-            else put<ROWS_A, COLS_A, SCALED>(i, rows_a, cols_a, pa, f0, f1);
+            const bool b = second(i);
+            float m = wave_max_abs(largest(x[i]));
+            if (__builtin_expect(m == INFINITY, 0)) m = wave_max_abs(largest_finite(x[i]));
+            if (SCALED && !b) m *= fabsf(f0 * f1);
+            int &least = QUADS % 256 == 0 ? run[b] : run[0];       // (a wavefront has either pieces of one tile only, or these in turn)
+            const int a = least = min(least, coarse_scale_of(m)), lane = threadIdx.x & 63;
+            if (lane < WAVE_ROWS / 8) powers[(b ? R / 8 : 0) + (__builtin_amdgcn_readfirstlane(row(i)) >> 3) + lane] = -a;
+            if (b) put<ROWS_B, COLS_B, false>(i, rows_b, cols_b, pow2(a), f0, f1);
+            else put<ROWS_A, COLS_A, SCALED>(i, rows_a, cols_a, pow2(a), f0, f1);
         }
     }
     template <bool ROWS, bool COLS, bool SCALED>
     __device__ __forceinline__ void put(const int i, u16 *rows, u16 *cols, const float p2, const float f0, const float f1) const {
+        if (!inside(i)) return;
         Planes w[4][2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             f32x4 v = x[i][j];
             if (SCALED) v = (v * f0) * f1;
-            v *= p2;
-            w[j][0] = split2(v.x, v.y);
-            w[j][1] = split2(v.z, v.w);
+            split4(v, p2, w[j][0], w[j][1]);
             if (ROWS) {
                 u16 *tr = rows + to_row[i] + j * (C + 8);
                 *reinterpret_cast<u32x2 *>(tr) = u32x2{w[j][0].h, w[j][1].h};
@@ -365,12 +401,24 @@ struct Stage {
         }
     }
 };
-// What find_largest left, over the workgroup: uniform.
-__device__ __forceinline__ f32x2 largest_of(const f32x2 *most) {
-    f32x2 m = most[0];
+// The negated powers of two of 32 rows, one for every eight: 2^n undoes them.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+struct Powers {
+    i32x4 n;
+    int lo, hi;              // uniform
+    __device__ __forceinline__ explicit Powers(const int *p) : n(*reinterpret_cast<const i32x4 *>(p)) {
+        lo = __builtin_amdgcn_readfirstlane(min(min(n.x, n.y), min(n.z, n.w)));
+        hi = __builtin_amdgcn_readfirstlane(max(max(n.x, n.y), max(n.z, n.w)));
+    }
+};
+// What is summed over rows with powers of their own is kept in units of 2^n, n the largest so far.  An operand's registers r
+// that stand for a row with a smaller one are taken down to it; returns the factor for what has been summed before.
+__device__ __forceinline__ float to_one_unit(const Powers &p, int &n, f32x16 &operand) {
+    const int was = n;
+    n = max(n, p.hi);
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = f32x2{fmaxf(m.x, most[w].x), fmaxf(m.y, most[w].y)};
-    return f32x2{__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m.x))), __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m.y)))};
+    for (int r = 0; r < 16; ++r) operand[r] *= __builtin_ldexpf(1.0f, p.n[r >> 2] - n);
+    return pow2(max(was - n, -200));
 }
 
 // Row of register r of a 32 x 32 accumulator in the lane's half of the wavefront (the column is lane % 32).

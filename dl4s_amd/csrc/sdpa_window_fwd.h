@@ -65,8 +65,8 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
                                                                              float *__restrict__ stats, const WindowGeometry g) {
     typedef Tile<BN, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
-    u16 *Ks = window_lds, *Vc = window_lds + 2 * T::ROWS_PLANE;
-    __shared__ f32x2 most[4];
+    u16 *Ks = window_lds, *Vc = Ks + 2 * T::ROWS_PLANE;
+    __shared__ __align__(16) int powers[2][BN / 8];        // [K, V]
 
     const int unit = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
     if (unit >= g.units) return;
@@ -76,15 +76,13 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;      // keys between them no query here sees
     Stage<BN, DT, VEC> kv(ks, g.d);
-    if (at.tiles > 0) {
-        kv.load(kp, vp, ks, at.key0(0), min(at.len, at.wp1 + 1), g.d, hide0, hide1);
-        kv.find_largest(most);
-    }
+    auto load = [&](const int i) { kv.load(kp, vp, ks, at.key0(i), min(at.len, at.wp1 + 1), g.d, hide0, hide1); };
+    if (at.tiles > 0) load(0);
 
     // scores in the base-2 exponent domain
     Frag qf[DT / 16];
     const float *qp = q + at.b * g.lq.b + at.h * g.lq.h + at.qc * g.lq.l;
-    const int aq = row_operand<DT>(qf, [&](const int c) { return load4(qp, c, g.d, VEC); }, g.rT, LOG2E);
+    const float unq = pow2(-row_operand<DT>(qf, [&](const int c) { return load4(qp, c, g.d, VEC); }, g.rT, LOG2E));
     const int p0 = g.w.q_offset + at.q0, p1 = g.w.q_offset + min(at.q0 + 31, g.Lq - 1), p = g.w.q_offset + at.qi;
     const bool idle = at.q0 >= g.Lq;
 
@@ -94,23 +92,14 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
     float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
-    int av = 126;                                          // o is in units of 2^-(av) of its values: the smallest power so far
+    int nv = -63;                                          // o is in units of 2^nv
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
-        const f32x2 top = largest_of(most);
-        const int ak = scale_of(top.x), av_new = min(av, scale_of(top.y));
-        if (av_new != av) {
-            const float f = pow2(max(av_new - av, -126));
-#pragma unroll
-            for (int t = 0; t < DT / 32; ++t) o[t] *= f;
-            av = av_new;
-        }
-        kv.template store<true, false, false, true, false>(Ks, nullptr, nullptr, Vc, pow2(ak), pow2(av));
+        kv.template store<true, false, false, true, false>(Ks, nullptr, nullptr, Vc, &powers[0][0]);
         __syncthreads();
-        if (i + 1 < at.tiles) kv.load(kp, vp, ks, at.key0(i + 1), min(at.len, at.wp1 + 1), g.d, hide0, hide1);
+        if (i + 1 < at.tiles) load(i + 1);
         const int t0 = at.key0(i);
-        const float f = pow2(max(-(aq + ak), -126));       // scores = accumulator * f
 #pragma unroll
         for (int sub = 0; sub < BN / 32; ++sub) {
             const int k0 = t0 + 32 * sub;
@@ -120,18 +109,25 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
             for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
             for (int st = 0; st < DT / 16; ++st) s = mma3(T::rows_frag(Ks, sub, st), qf[st], s);
+            const i32x4 nk = *reinterpret_cast<const i32x4 *>(&powers[0][4 * sub]);
+            const Powers vs(&powers[1][4 * sub]);
+            settle(s);
             if (!tile_open(g.w, p0, p1, k0, at.len)) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = sees(g.w, p, k0 + acc_row(r) + 4 * half, at.len) ? s[r] : -INFINITY;
             }
-            float tmax = s[0];
+            // scores = accumulators * f, one factor for every eight keys
+            float f[4], tmax = -INFINITY;
 #pragma unroll
-            for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[r]);
-            tmax = max_halves(tmax) * f;
+            for (int x = 0; x < 4; ++x) {
+                f[x] = __builtin_ldexpf(unq, nk[x]);
+                tmax = fmaxf(tmax, fmaxf(fmaxf(s[4 * x], s[4 * x + 1]), fmaxf(s[4 * x + 2], s[4 * x + 3])) * f[x]);
+            }
             // the reference maximum moves, and the sums are rescaled, only when a weight would pass 2^8 (x 2^7): any factor
             // left in the weights of a row cancels in the division by their sum
             if (__any(tmax - m_run > 8.0f)) {
-                const float m_new = fmaxf(m_run, tmax);
+                tmax = max_halves(tmax);
+                const float m_new = tmax - m_run > 8.0f ? tmax : m_run;
                 const float alpha = m_run == m_new ? 1.0f : exp2_fast(m_run - m_new);
                 m_run = m_new;
                 m_use = m_new == -INFINITY ? 0.f : m_new - 7.0f;
@@ -141,25 +137,33 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[r] = exp2_fast(__builtin_fmaf(s[r], f, -m_use));
+                s[r] = exp2_fast(__builtin_fmaf(s[r], f[r >> 2], -m_use));
                 l_run += s[r];
+            }
+            if (vs.lo != nv || vs.hi != nv) {
+                const float unit = to_one_unit(vs, nv, s);
+#pragma unroll
+                for (int t = 0; t < DT / 32; ++t) o[t] *= unit;
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const Frag pf = acc_frag(s, st);
+                Frag vf[DT / 32];
 #pragma unroll
-                for (int t = 0; t < DT / 32; ++t) o[t] = mma3(T::cols_frag(Vc, t, 2 * sub + st), pf, o[t]);
+                for (int t = 0; t < DT / 32; ++t) vf[t] = T::cols_frag(Vc, t, 2 * sub + st);
+                mma3(o, vf, pf);
             }
         }
-        if (i + 1 < at.tiles) kv.find_largest(most);
     }
 
+#pragma unroll
+    for (int t = 0; t < DT / 32; ++t) settle(o[t]);
     if (at.qi >= g.Lq) return;
     const float l = sum_halves(l_run);
     // a row that saw no key: zeros
     const Range see = visible_keys(g.w, at.b, at.qi, g.Lk);
     const float inv = see.first + (see.hi - see.lo) > 0 ? 1.0f / l : 0.f;
-    const float unscale = pow2(-av);
+    const float unscale = pow2(nv);
     float *op = out + at.b * g.lq.b + at.h * g.lq.h + at.qi * g.lq.l;
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
