@@ -7,10 +7,12 @@
 //
 // Bound: reading the logits once from HBM (the gradient: reading and writing them once).  token_logprobs_f32 makes one pass:
 // every lane keeps a running maximum m, l = sum exp(z - m) and u = sum exp(z - m) (z - m) of its own values, in fp32, and a
-// wavefront keeps the alternatives as one sorted list, the i-th best in lane i.  A value and its token are one 64-bit
-// integer that orders them, so the list is exact and does not depend on who was ready first.  After the first tile few
-// values beat the k-th best (about k ln(n / 1024) of n in random order), each is found by a ballot and inserted by shifting
-// the lanes behind it; the wavefronts of a workgroup share the highest k-th best found so far.
+// wavefront keeps the alternatives it met as one sorted list, the i-th best in lane i.  A value and its token are one 64-bit
+// integer that orders them, so the result is exact and does not depend on who was ready first.  Only values above a bound
+// are looked at: the k-th largest of the maxima that 128 groups of lanes have seen so far, k values that are really there.  The
+// workgroup renews it after 1, 2, 4, 8 ... tiles, so about k values per doubling of what has been read come through; each is
+// found by a ballot and inserted by shifting the lanes behind it.  What is left at the end, a few more than k values, is put in
+// order by counting.
 #include "common.h"
 
 #include <algorithm>
@@ -85,14 +87,20 @@ __device__ __forceinline__ void row_results(const Outputs &o, const long long ro
     if (o.entropy) o.entropy[row] = H;
     if (o.stats) { o.stats[3 * row] = s.m; o.stats[3 * row + 1] = L; o.stats[3 * row + 2] = H; }
 }
-// The `top` largest of `count` keys in LDS (0 = none) as outputs, or as keys: each is put where its rank says.
-__device__ __forceinline__ void rank_keys(const u64 *keys, const int count, const int top, const Outputs *o, const long long row, const Sums s,
+// The `top` largest of `count` keys in LDS (0 = none) as outputs, or as keys: each is put where its rank says.  The keys are
+// read in pieces of eight: the list is filled up with zeros.
+__device__ __forceinline__ void rank_keys(u64 *keys, const int count, const int top, const Outputs *o, const long long row, const Sums s,
                                           u64 *to) {
+    if (threadIdx.x < 8) keys[count + threadIdx.x] = 0;
+    __syncthreads();
     for (int e = threadIdx.x; e < count; e += blockDim.x) {
         const u64 key = keys[e];
         if (key == 0) continue;
         int rank = 0;
-        for (int j = 0; j < count; ++j) rank += keys[j] > key;
+        for (int j = 0; j < count; j += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rank += keys[j + i] > key;
+        }
         if (rank >= top) continue;
         if (to) to[rank] = key;
         else {
@@ -102,51 +110,91 @@ __device__ __forceinline__ void rank_keys(const u64 *keys, const int count, cons
     }
 }
 
+// Largest of the GS lanes (2 or 8, consecutive) that hold the lane.
+template <int CTRL>
+__device__ __forceinline__ float max_lanes(const float v) {
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)));
+}
+template <int GS>
+__device__ __forceinline__ float group_max(float v) {
+    v = max_lanes<0xB1>(v);            // quad_perm [1,0,3,2]
+    if (GS == 8) {
+        v = max_lanes<0x4E>(v);        // quad_perm [2,3,0,1]
+        v = max_lanes<0x141>(v);       // row_half_mirror
+    }
+    return v;
+}
+// A key below which no key of the `top` largest lies, from 128 values of different tokens (-inf: no token), two per lane: the
+// upper 16 bits of the top-th largest, found bit by bit.
+__device__ __forceinline__ u64 lower_bound(const float v, const float w, const int top) {
+    const unsigned u = (unsigned)(order_key(v, 0) >> 32), y = (unsigned)(order_key(w, 0) >> 32);
+    unsigned prefix = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const unsigned with = prefix | (1u << bit);
+        if (__popcll(__ballot(u >= with)) + __popcll(__ballot(y >= with)) >= top) prefix = with;
+    }
+    return prefix <= 0x007FFFFFu ? 0 : ((u64)prefix << 32) - 1;          // not above -inf: no bound
+}
+
 // One workgroup per row, or per part of a row (blockIdx.x); parts leave [top keys][m, l, u] in scratch for the merge.
 template <int NW, bool TOP>
 __global__ __launch_bounds__(NW * 64) void token_logprobs_f32(const float *__restrict__ x, const long long n, const long long stride,
                                                                const float t, const Outputs out, const int parts, u64 *partial) {
+    constexpr int GS = NW / 2, GROUPS = 64 / GS;                         // groups of lanes: 128 in the workgroup
     __shared__ Sums sums[NW];
-    __shared__ u64 keys[TOP ? NW * MAX_TOP : 1], bar;
+    __shared__ u64 keys[TOP ? NW * MAX_TOP + 8 : 1], bar;
+    __shared__ float seen[2][TOP ? 128 : 1];
+    __shared__ int kept;
     const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
     const int part = blockIdx.x;
     const float *xr = x + row * stride;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (TOP) {
-        if (threadIdx.x == 0) bar = 0;
-        __syncthreads();
-    }
+    if (TOP && threadIdx.x == 0) { bar = 0; kept = 0; }
 
     // granules of 16 bytes: granule g holds elements 4 g - before .. + 3 of the row
     const int before = (int)((reinterpret_cast<uintptr_t>(xr) >> 2) & 3);
     const long long granules = (n + before + 3) / 4, share = ((granules + parts - 1) / parts + 255) / 256 * 256;
     const long long g0 = part * share, g1 = min(granules, g0 + share);
     const float *xg = xr - before;
+    const int tiles = (int)((max(g1 - g0, 0ll) + 256 * NW - 1) / (256 * NW));
 
-    Sums s = {-INFINITY, 0.f, 0.f};
-    u64 list = 0, tau = 0;
-    bool filled = false;
-    for (long long base = g0 + 256 * wave; base < g1; base += 256 * NW) {
-        float z[16];
-        if (4 * base >= before && 4 * (base + 256) - before <= n) {          // no granule is cut by the row's ends
+    // sixteen values of the lane; what lies outside the row is -inf
+    auto load = [&](const long long base, f32x4 (&v)[4]) {
+        if (base >= g1) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(xg + 4 * (base + 64 * i + lane)));
+            for (int i = 0; i < 4; ++i) v[i] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        } else if (4 * base >= before && 4 * (base + 256) - before <= n) {   // no granule is cut by the row's ends
 #pragma unroll
-                for (int c = 0; c < 4; ++c) z[4 * i + c] = scaled(v[c], t);
-            }
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(xg + 4 * (base + 64 * i + lane)));
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const long long j = 4 * (base + 64 * i + lane) - before + c;
-                    z[4 * i + c] = j >= 0 && j < n ? scaled(xr[j], t) : -INFINITY;
+                    v[i][c] = j >= 0 && j < n ? xr[j] : (t < 0.f ? INFINITY : -INFINITY);
                 }
         }
-        float mx = z[0];
+    };
+
+    Sums s = {-INFINITY, 0.f, 0.f};
+    u64 list = 0, tau = 0;                                               // keys above tau are wanted
+    f32x4 next[4];
+    if (TOP) load(g0 + 256 * wave, next);                                // (the other form has nothing to do that would hold up its loads)
+    for (int tile = 0; tile < tiles; ++tile) {
+        const long long base = g0 + 256 * (wave + (long long)NW * tile);
+        float z[16], mx = -INFINITY;
+        if (!TOP) load(base, next);
 #pragma unroll
-        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, z[e]);
+        for (int e = 0; e < 16; ++e) z[e] = scaled(next[e >> 2][e & 3], t);
+        if (base >= g1) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) z[e] = -INFINITY;
+        }
+        if (TOP) load(base + 256 * NW, next);
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) mx = fmaxf(fmaxf(mx, z[e]), z[e + 1]);
         const float M = fmaxf(s.m, mx);
         const float mu = M == -INFINITY ? 0.f : M;
         s = rescaled(s, M);
@@ -157,40 +205,23 @@ __global__ __launch_bounds__(NW * 64) void token_logprobs_f32(const float *__res
             s.u += p * fmaxf(y, -1e4f);                                      // p = 0 far below: 0 * -inf is no term
         }
         if (TOP) {
-            // keys of the tile in registers again: a token outside the row has none
-            auto key_of = [&](const int e) {
-                const long long j = 4 * (base + 64 * (e >> 2) + lane) - before + (e & 3);
-                return j >= 0 && j < n ? order_key(z[e], (unsigned)j) : 0;
-            };
-            const u64 others = __hip_atomic_load(&bar, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            tau = others > tau ? others : tau;
-            // (tau below every value there is, NaN included, while its high word is 0)
-            if ((tau >> 32) == 0 || __any(mx >= key_value(tau))) {
-                unsigned taken = 0;                                          // the value of this lane that the list already holds
-                if (!filled) {
-                    // the first tile: every lane's best value, sorted by counting how many lanes have a better one
-                    filled = true;
-                    u64 best = 0;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const u64 key = key_of(e);
-                        if (key > best) { best = key; taken = 1u << e; }
-                    }
-                    int rank = 0;
-#pragma unroll 16
-                    for (int i = 0; i < 64; ++i) {
-                        const u64 other = lane_key(best, i);
-                        rank += other > best || (other == best && i < lane);    // (equal only where there is no token)
-                    }
-                    const unsigned lo = (unsigned)__builtin_amdgcn_ds_permute(rank << 2, (int)(unsigned)best);
-                    const unsigned hi = (unsigned)__builtin_amdgcn_ds_permute(rank << 2, (int)(best >> 32));
-                    list = ((u64)hi << 32) | lo;
-                    const u64 kth = lane_key(list, out.top - 1);
-                    tau = kth > tau ? kth : tau;
-                }
+            if ((tile & (tile - 1)) == 0) {                                  // the same tiles for every wavefront
+                const int turn = (tile == 0 ? 0 : __builtin_ctz(tile) + 1) & 1;
+                const float gm = group_max<GS>(s.m);
+                if (lane % GS == 0) seen[turn][wave * GROUPS + lane / GS] = gm;
+                __syncthreads();
+                const u64 low = lower_bound(seen[turn][lane], seen[turn][64 + lane], out.top);
+                tau = low > tau ? low : tau;
+            }
+            float tau_value = (tau >> 32) == 0 ? -INFINITY : key_value(tau);
+            if (__any(!(mx < tau_value)) && base < g1) {
+                const u64 others = __hip_atomic_load(&bar, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (others > tau) { tau = others; tau_value = key_value(tau); }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const u64 key = (taken >> e) & 1 ? 0 : key_of(e);
+                    if (!__any(!(z[e] < tau_value))) continue;               // (a NaN passes: its key decides)
+                    const long long j = 4 * (base + 64 * (e >> 2) + lane) - before + (e & 3);
+                    const u64 key = j >= 0 && j < n ? order_key(z[e], (unsigned)j) : 0;
                     u64 better = __ballot(key > tau);
                     while (better) {
                         const int from = __builtin_ctzll(better);
@@ -199,7 +230,7 @@ __global__ __launch_bounds__(NW * 64) void token_logprobs_f32(const float *__res
                         const u64 shifted = key_before(list);
                         list = lane < pos ? list : (lane == pos ? add : shifted);
                         const u64 kth = lane_key(list, out.top - 1);
-                        tau = kth > tau ? kth : tau;
+                        if (kth > tau) { tau = kth; tau_value = key_value(tau); }
                         better &= __ballot(key > tau) & ~(1ull << from);
                     }
                 }
@@ -213,8 +244,19 @@ __global__ __launch_bounds__(NW * 64) void token_logprobs_f32(const float *__res
     s.l = dl4s::wave_sum(s.l);
     s.u = dl4s::wave_sum(s.u);
     if (lane == 0) sums[wave] = s;
-    if (TOP && lane < out.top) keys[wave * out.top + lane] = list;
     __syncthreads();
+    int count = 0;
+    if (TOP) {
+        // bar is at most the top-th largest key of the row: what is not below it goes on
+        const bool keep = lane < out.top && list != 0 && list >= bar;
+        const u64 keeping = __ballot(keep);
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&kept, __popcll(keeping));
+        at = __builtin_amdgcn_readfirstlane(at) + __popcll(keeping & ((1ull << lane) - 1));
+        if (keep) keys[at] = list;
+        __syncthreads();
+        count = kept;
+    }
     float Mall = sums[0].m;
 #pragma unroll
     for (int w = 1; w < NW; ++w) Mall = fmaxf(Mall, sums[w].m);
@@ -235,18 +277,16 @@ __global__ __launch_bounds__(NW * 64) void token_logprobs_f32(const float *__res
         }
     }
     if (TOP) {
-        if (rec) {                     // a part may hold fewer keys than asked for
+        if (rec)                       // a part may hold fewer keys than asked for
             for (int e = threadIdx.x; e < out.top; e += NW * 64) rec[e] = 0;
-            __syncthreads();
-        }
-        rank_keys(keys, NW * out.top, out.top, &out, row, all, rec);
+        rank_keys(keys, count, out.top, &out, row, all, rec);
     }
 }
 
 // Joins the parts of a row: one workgroup per row.
 __global__ __launch_bounds__(256) void token_logprobs_merge_f32(const float *__restrict__ x, const long long n, const long long stride,
                                                                  const float t, const Outputs out, const int parts, const u64 *partial) {
-    __shared__ u64 keys[MERGE_KEYS];
+    __shared__ u64 keys[MERGE_KEYS + 8];
     const long long row = blockIdx.x;
     const u64 *rec = partial + row * parts * (out.top + 2);
     Sums all = {-INFINITY, 0.f, 0.f};
@@ -342,11 +382,13 @@ int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t 
                  (long long)top_k, MAX_TOP);
     DL4S_REQUIRE(top_k <= n, DL4S_HIP_ESHAPE, "token_logprobs: %lld alternatives of %lld tokens", (long long)top_k, (long long)n);
     DL4S_REQUIRE(top_k == 0 || (top_logprobs && top_tokens), DL4S_HIP_EINVALID_ARG, "token_logprobs: NULL output for the alternatives");
-    // Few rows: 16 wavefronts to a row, and long rows in parts of at least 16384 tokens (a wavefront's tile each) until every
-    // compute unit has one.  Many rows: 4 wavefronts, whose lists of alternatives are filled over longer pieces.
-    const bool few = rows <= ctx->cu_count;
+    // 16 wavefronts to a row where there are too few rows to fill the GPU with four: up to one row to a compute unit, without
+    // alternatives up to four (with them the renewed bound has 16 wavefronts wait for each other: 1000 rows of 50000 tokens and
+    // 20 alternatives 79 us, with 4 wavefronts 52).  Up to one row to a compute unit long rows come in parts, too, of at least
+    // 16384 tokens (a tile for each wavefront).
+    const bool few = rows <= (top_k ? 1 : 4) * ctx->cu_count;
     int64_t parts = 1;
-    if (few) {
+    if (rows <= ctx->cu_count) {
         parts = std::min<int64_t>(n / 16384, ctx->cu_count / rows);
         parts = std::min<int64_t>(parts, top_k ? MERGE_KEYS / top_k : 64);
         parts = std::max<int64_t>(parts, 1);
