@@ -336,7 +336,7 @@ int few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, 
     // 512 keys one workgroup reads them all, and a workgroup has at least 256 keys.
     const int NW = 8;
     const int64_t most = std::min<int64_t>(Lk, (int64_t)w.window + Lq - 1 + w.sinks), blocks = pairs * ((a.cols + 15) / 16);
-    int64_t ns = most <= 512 ? 1 : std::min((ctx->cu_count + blocks - 1) / blocks, (most + 255) / 256);
+    int64_t ns = most <= 512 ? 1 : std::min<int64_t>(MAX_SPLIT, std::min((ctx->cu_count + blocks - 1) / blocks, (most + 255) / 256));
     a.chunk = (int)std::max<int64_t>(16, ((most + ns - 1) / ns + 15) / 16 * 16);
     a.nsplit = (int)std::max<int64_t>(1, (most + a.chunk - 1) / a.chunk);
     a.partial = nullptr;
@@ -352,7 +352,7 @@ int few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, 
     else if (d <= 128) rc = launch_few_rows<128, NW>(ctx, q, k, v, out, stats, a, pairs);
     else rc = launch_few_rows<256, NW>(ctx, q, k, v, out, stats, a, pairs);
     if (rc || a.nsplit == 1) return rc;
-    hipLaunchKernelGGL(sdpa_window_merge_f32, dim3(a.cols, (unsigned)pairs), dim3(256), 0, ctx->stream, out, stats, a);
+    hipLaunchKernelGGL(sdpa_window_merge_f32, dim3(a.cols, (unsigned)pairs), dim3(MAX_SPLIT), 0, ctx->stream, out, stats, a);
     return dl4s::launch_status("sdpa_window_merge_f32");
 }
 

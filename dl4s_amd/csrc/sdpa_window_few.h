@@ -27,7 +27,7 @@ struct FewArgs {
 };
 
 template <int DT, int NW>
-__global__ __launch_bounds__(NW * 64, DT <= 64 ? 4 : (DT <= 128 ? 2 : 1)) void sdpa_window_few_f32(
+__global__ __launch_bounds__(NW * 64, DT <= 64 ? 3 : (DT <= 128 ? 2 : 1)) void sdpa_window_few_f32(
     const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v, float *__restrict__ out,
     float *__restrict__ stats, const FewArgs a) {
     extern __shared__ __align__(16) float few_lds[];
@@ -62,26 +62,35 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 4 : (DT <= 128 ? 2 : 1)) void s
         for (int e = 0; e < 4; ++e) o[j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
 
-    for (int x = x0 + 16 * wave; x < x1; x += 16 * NW) {
-        auto key_at = [&](const int i) { const int y = min(x + i, x1 - 1); return y < first ? y : lo + y - first; };
-        f32x4 kk[DT / 16], vv[4][DT / 64];
-        const float *kr = kp + key_at(ln) * a.lk.l;
+    // a row's four floats, once: nothing here is read again
+    auto stream4 = [&](const float *row, const int c) -> f32x4 {
+        if (!a.vec) return load4(row, c, a.d, false);
+        return c < a.d ? __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(row + c)) : f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    struct Keys {
+        f32x4 k[DT / 16], v[4][DT / 64];
+    };
+    auto key_at = [&](const int i) { const int y = min(i, x1 - 1); return y < first ? y : lo + y - first; };
+    auto fetch = [&](Keys &f, const int x) {
+        const float *kr = kp + key_at(x + ln) * a.lk.l;
 #pragma unroll
-        for (int s = 0; s < DT / 16; ++s) kk[s] = load4(kr, 16 * s + 4 * quad, a.d, a.vec);
+        for (int s = 0; s < DT / 16; ++s) f.k[s] = stream4(kr, 16 * s + 4 * quad);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float *vr = vp + key_at(4 * quad + r) * a.lk.l;
+            const float *vr = vp + key_at(x + 4 * quad + r) * a.lk.l;
 #pragma unroll
-            for (int j = 0; j < DT / 64; ++j) vv[r][j] = load4(vr, 64 * j + 4 * ln, a.d, a.vec);
+            for (int j = 0; j < DT / 64; ++j) f.v[r][j] = stream4(vr, 64 * j + 4 * ln);
         }
+    };
+    auto attend = [&](const Keys &f, const int x) {
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < DT / 16; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[t][e], qf[4 * t + e], s, 0, 0, 0);
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(f.k[t][e], qf[4 * t + e], s, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int j = key_at(4 * quad + r);
+            const int j = key_at(x + 4 * quad + r);
             s[r] = ((x + 4 * quad + r < x1) & sees(a.w, p, j, len)) ? s[r] : -INFINITY;
         }
         const float tmax = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
@@ -106,7 +115,27 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 4 : (DT <= 128 ? 2 : 1)) void s
 #pragma unroll
             for (int j = 0; j < DT / 64; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[r][j][e], s[r], o[j][e], 0, 0, 0);
+                for (int e = 0; e < 4; ++e) o[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.v[r][j][e], s[r], o[j][e], 0, 0, 0);
+        }
+    };
+    // the next 16 keys are on their way while these are worked on (rows above 128 columns: no registers for that)
+    constexpr int STEP = 16 * NW;
+    int x = x0 + 16 * wave;
+    if (DT <= 128) {
+        Keys f0, f1;
+        if (x < x1) fetch(f0, x);
+        for (; x < x1; x += 2 * STEP) {
+            fetch(f1, x + STEP);
+            attend(f0, x);
+            if (x + STEP >= x1) break;
+            fetch(f0, x + 2 * STEP);
+            attend(f1, x + STEP);
+        }
+    } else {
+        Keys f;
+        for (; x < x1; x += STEP) {
+            fetch(f, x);
+            attend(f, x);
         }
     }
     l_run += __shfl_xor(l_run, 16, 64);
@@ -159,24 +188,44 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 4 : (DT <= 128 ? 2 : 1)) void s
     }
 }
 
-// Merges the partial results of one query row: one workgroup per row, a thread per column.
-__global__ __launch_bounds__(256) void sdpa_window_merge_f32(float *__restrict__ out, float *__restrict__ stats, const FewArgs a) {
-    const int row = blockIdx.x, pair = blockIdx.y, x = threadIdx.x;
+constexpr int MAX_SPLIT = 256;
+
+// Merges the partial results of one query row: one workgroup per row.  A thread has one part's maximum and sum, then one column of
+// all parts, whose loads do not wait for each other.
+__global__ __launch_bounds__(MAX_SPLIT) void sdpa_window_merge_f32(float *__restrict__ out, float *__restrict__ stats, const FewArgs a) {
+    __shared__ float factor[MAX_SPLIT], most[4], total[4];
+    const int row = blockIdx.x, pair = blockIdx.y, x = threadIdx.x, wave = x >> 6;
     const int hk = pair % a.Hkv, b = pair / a.Hkv, h = hk * a.group + row / a.Lq, i = row % a.Lq;
     const long long step = (long long)a.cols * (a.d + 2);
     const float *rec = a.partial + ((long long)pair * a.nsplit * a.cols + row) * (a.d + 2);
-    float M = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, rec[s * step + a.d]);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, O = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float m = rec[s * step + a.d], f = m == -INFINITY ? 1.0f : exp2_fast(m - Mu);
-        L += rec[s * step + a.d + 1] * f;
-        if (x < a.d) O += rec[s * step + x] * f;
-    }
+    const float m = x < a.nsplit ? rec[x * step + a.d] : -INFINITY, l = x < a.nsplit ? rec[x * step + a.d + 1] : 0.f;
+    float M = m;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if ((x & 63) == 0) most[wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    const float Mu = M == -INFINITY ? 0.f : M, f = m == -INFINITY ? 1.0f : exp2_fast(m - Mu);
+    factor[x] = f;
+    const float part = dl4s::wave_sum(l * f);
+    if ((x & 63) == 0) total[wave] = part;
+    __syncthreads();
+    const float L = (total[0] + total[1]) + (total[2] + total[3]);
     const Range r = visible_keys(a.w, b, i, a.Lk);
     const float inv = r.first + (r.hi - r.lo) > 0 ? 1.0f / L : 0.f;
-    if (x < a.d) out[b * a.lq.b + h * a.lq.h + i * a.lq.l + x] = O * inv;
+    if (x < a.d) {
+        float O = 0.f;
+        int s = 0;
+        for (; s + 8 <= a.nsplit; s += 8) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = rec[(s + e) * step + x];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) O += p[e] * factor[s + e];
+        }
+        for (; s < a.nsplit; ++s) O += rec[s * step + x] * factor[s];
+        out[b * a.lq.b + h * a.lq.h + i * a.lq.l + x] = O * inv;
+    }
     if (stats && x == 0) {
         const long long at = 2 * (((long long)b * a.H + h) * a.Lq + i);
         stats[at] = Mu;
