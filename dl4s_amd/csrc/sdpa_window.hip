@@ -249,22 +249,31 @@ int launch_fwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const fl
     return launch_fwd<128, 32, VEC>(ctx, q, k, v, out, stats, g);
 }
 
-// Deals the key blocks to workgroups.  A block that every later query sees (first keys) gets about as many query tiles per
-// workgroup as a block that only its window's queries see, and all get more workgroups while there are fewer than two per
-// compute unit; at most 2048 workgroups leave partial sums.
+// Deals the key blocks to workgroups, of which a compute unit has one at a time.  The blocks without first keys are cut into as
+// many pieces as make the longest queue of a compute unit shortest (in query tiles: a workgroup costs about one more, a
+// second launch that adds up partial sums about three, and their way through memory); those with first keys, which
+// every later query sees, into enough pieces to give every compute unit one.  At most 2048 workgroups leave partial sums.
 KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B) {
     KeyBlocks kb;
     kb.pairs = (int)(B * g.Hkv);
     kb.blocks = (g.Lk + 127) / 128;
     kb.sink_blocks = std::min(kb.blocks, (g.w.sinks + 127) / 128);
-    const long long tiles = (g.Lq + 31) / 32, near = std::min<long long>(tiles, (g.w.window + 127ll + 31) / 32 + 1);
+    const long long cus = ctx->cu_count, tiles = (g.Lq + 31) / 32, near = std::min<long long>(tiles, (g.w.window + 127ll + 31) / 32 + 1);
     const long long n[2] = {tiles * g.group, near * g.group}, count[2] = {(long long)kb.pairs * kb.sink_blocks, (long long)kb.pairs * (kb.blocks - kb.sink_blocks)};
-    const long long fill = (2ll * ctx->cu_count + kb.pairs * (long long)kb.blocks - 1) / (kb.pairs * (long long)kb.blocks);
     long long floats = 0;
     for (int c = 0; c < 2; ++c) {
-        long long chunks = std::max(fill, c ? 1 : (tiles + near - 1) / near);
-        chunks = std::min(chunks, std::max(1ll, n[c] / 4));
-        chunks = std::min(chunks, std::max(1ll, 2048 / std::max(1ll, count[c])));
+        const long long most = std::max(1ll, std::min(n[c] / 4, 2048 / std::max(1ll, count[c])));
+        long long chunks = 1;
+        if (c == 0) {
+            chunks = std::min(most, std::max(1ll, (cus + count[0] - 1) / std::max(1ll, count[0])));
+        } else {
+            double best = 0;
+            for (long long x = 1; x <= std::min(most, 8ll); ++x) {
+                const double queue = (double)((count[1] * x + cus - 1) / cus) * (double)((n[1] + x - 1) / x + 1);
+                const double cost = queue + (x > 1 ? 3.0 + (double)(count[1] * x) * g.d * 2e-4 : 0.0);   // 2 KiB of d, at 5 TB/s and 2 us a tile
+                if (x == 1 || cost < best) { best = cost; chunks = x; }
+            }
+        }
         kb.chunks[c] = (int)chunks;
         kb.units[c] = (int)(count[c] * chunks);
         kb.per_xcd[c] = (kb.units[c] + 7) / 8;
@@ -279,7 +288,7 @@ template <int DT, bool VEC>
 int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats, const float *dout,
                float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
     typedef Tile<32, DT> T;
-    const size_t lds_q = 2 * 2 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 4 * (T::ROWS_PLANE + T::COLS_PLANE);
+    const size_t lds_q = 2 * 2 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 4 * (T::ROWS_PLANE + T::COLS_PLANE) + 16384;
     int rc = lds_limit(ctx, dl4s::LDS_WINDOW, 2 * (DT / 32 - 1) + VEC, sdpa_window_dq_f32<DT, VEC>, lds_q);
     if (!rc) rc = lds_limit(ctx, dl4s::LDS_WINDOW_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dkv_f32<DT, VEC>, lds_k);
     if (rc) return rc;
@@ -289,7 +298,7 @@ int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v
         if (rc) return rc;
     }
     if (kb.pairs && kb.blocks) {
-        hipLaunchKernelGGL((sdpa_window_dkv_f32<DT, VEC>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1])), dim3(256), lds_k, ctx->stream, q, k, v, stats,
+        hipLaunchKernelGGL((sdpa_window_dkv_f32<DT, VEC>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1])), dim3(512), lds_k, ctx->stream, q, k, v, stats,
                            dout, delta, dk, dv, g, kb);
         rc = dl4s::launch_status("sdpa_window_dkv_f32");
         for (int c = 0; c < 2 && !rc; ++c) {

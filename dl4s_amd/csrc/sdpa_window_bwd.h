@@ -3,12 +3,14 @@
 //   sdpa_window_dq_f32   workgroups, tiles and operand order of the forward kernel:
 //     S^T = K . Q^T, dP^T = V . dO^T, dS^T = w (dP^T - delta), dQ^T += K^T . dS^T; it also forms delta = dO . out per row
 //     and leaves it in scratch for the other kernel.
-//   sdpa_window_dkv_f32  one workgroup = 128 keys of a key head (a wavefront holds 32 keys as columns, K and V in registers)
-//     over 32-row query tiles of all query heads of the group:
-//     S = Q . K^T, dP = dO . V^T, dV^T += dO^T . w, dK^T += Q^T . dS
-//     so shared key heads are summed in the accumulators, in a fixed order, without atomics.  Key blocks that hold visible
+//   sdpa_window_dkv_f32  one workgroup = 8 wavefronts = 128 keys of a key head over 32-row query tiles of all query heads of the
+//     group.  Two wavefronts share 32 keys (the columns of their accumulators): one holds K and forms S = Q . K^T, the weights
+//     w, and dV^T += dO^T . w, the other holds V and forms dP = dO . V^T and, with the weights it gets through LDS,
+//     dK^T += Q^T . dS.  That halves what a wavefront keeps in registers, so two run on a SIMD at every head dim (one
+//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes DKV_US at B2 H16/4 L4096 d96 window 777).
+//     Shared key heads are summed in the accumulators, in a fixed order, without atomics.  Key blocks that hold visible
 //     first keys are seen by every later query: their query tiles are dealt to several workgroups whose partial sums a
-//     last kernel adds up in order; so are all blocks when there are too few of them to fill the GPU.
+//     last kernel adds up in order; so are all blocks where that shortens the longest queue of a compute unit.
 // The size of dS, and of the weights a key gets, is not known beforehand: as operands they carry a power of two per column
 // (query or key), set by the first tile so that the largest value there is 2^8 and lowered, with the accumulators, when a
 // later one would pass 2^15.
@@ -76,7 +78,7 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
 
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;
-    Stage<32, DT, VEC> kv(ks, g.d);
+    Stage<32, DT, VEC> kv(ks, g.d, threadIdx.x);
     auto load = [&](const int i) { kv.load(kp, vp, ks, at.key0(i), min(at.len, at.wp1 + 1), g.d, hide0, hide1); };
     if (at.tiles > 0) load(0);
 
@@ -168,9 +170,10 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
         }
 }
 
-// How the key blocks (128 keys) of all (batch, key head) pairs are dealt to workgroups: those that hold visible first keys,
-// then the others; each in `chunks` equal pieces of its query tiles.  Workgroup ids of a class go round the XCDs so that
-// consecutive pieces of work share one XCD's L2.
+// How the key blocks (128 keys) of all (batch, key head) pairs are dealt to workgroups: class 0 are those that hold visible
+// first keys, class 1 the others; each in `chunks` equal pieces of its query tiles.  The pieces of class 1 are started
+// first, the shorter ones of class 0 fill up.  Workgroup ids of a class go round the XCDs so that consecutive pieces of
+// work share one XCD's L2.
 struct KeyBlocks {
     int pairs, blocks, sink_blocks;
     int chunks[2];                   // [0] blocks with first keys, [1] the others
@@ -186,28 +189,29 @@ __device__ __forceinline__ float *partial_sums(const KeyBlocks &kb, const int pa
 }
 
 template <int DT, bool VEC>
-__global__ __launch_bounds__(256, DT <= 64 ? 2 : 1) void sdpa_window_dkv_f32(const float *__restrict__ q, const float *__restrict__ k,
-                                                                             const float *__restrict__ v,
-                                                                             const float *__restrict__ stats,
-                                                                             const float *__restrict__ dout,
-                                                                             const float *__restrict__ delta, float *__restrict__ dk,
-                                                                             float *__restrict__ dv, const WindowGeometry g,
-                                                                             const KeyBlocks kb) {
+__global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__restrict__ q, const float *__restrict__ k,
+                                                               const float *__restrict__ v, const float *__restrict__ stats,
+                                                               const float *__restrict__ dout, const float *__restrict__ delta,
+                                                               float *__restrict__ dk, float *__restrict__ dv, const WindowGeometry g,
+                                                               const KeyBlocks kb) {
     typedef Tile<32, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
     u16 *Qs = window_lds, *Gs = Qs + 2 * T::ROWS_PLANE, *Qc = Gs + 2 * T::ROWS_PLANE, *Gc = Qc + 2 * T::COLS_PLANE;
+    f32x4 *weights = reinterpret_cast<f32x4 *>(Gc + 2 * T::COLS_PLANE);        // [pair of wavefronts][4][lane]
     __shared__ __align__(16) float rowv[96];               // [3][32]: m, 2^13 / l, delta of the tile's queries
     __shared__ __align__(16) int powers[2][4];             // [Q, dO]
 
-    int id = blockIdx.x, cl = 0;
-    if (id >= 8 * kb.per_xcd[0]) { id -= 8 * kb.per_xcd[0]; cl = 1; }
+    int id = blockIdx.x, cl = 1;
+    if (id >= 8 * kb.per_xcd[1]) { id -= 8 * kb.per_xcd[1]; cl = 0; }
     const int unit = (id & 7) * kb.per_xcd[cl] + (id >> 3);
     if (unit >= kb.units[cl]) return;
     const int chunk = unit % kb.chunks[cl], in_class = cl ? kb.blocks - kb.sink_blocks : kb.sink_blocks;
     const int block = unit / kb.chunks[cl] % in_class + (cl ? kb.sink_blocks : 0), pair = unit / kb.chunks[cl] / in_class;
     const int hk = pair % g.Hkv, b = pair / g.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, ln = lane & 31;
-    const int b0 = block * 128, k0 = b0 + wave * 32, key = k0 + ln;
+    const int two = wave & 3;
+    const bool values = wave >= 4;                         // holds V, forms dP and dK; the other holds K, forms w and dV
+    const int b0 = block * 128, k0 = b0 + two * 32, key = k0 + ln;
     const int len = valid_keys(g.w, b, g.Lk);
 
     // query tiles that can see the block: from the first key's position to the window's end behind the last key.  Queries that
@@ -218,7 +222,8 @@ __global__ __launch_bounds__(256, DT <= 64 ? 2 : 1) void sdpa_window_dkv_f32(con
     const int per_head = b0 < len && t1 > t0 ? t1 - t0 : 0;
     const int all = per_head * g.group, from = (int)((long long)all * chunk / kb.chunks[cl]), to = (int)((long long)all * (chunk + 1) / kb.chunks[cl]);
 
-    Stage<32, DT, VEC> qg((int)g.lq.l, g.d);
+    // (wavefronts take pieces of the tiles in the order 0, 4, 1, 5, ...: where there are fewer pieces, both kinds get some)
+    Stage<32, DT, VEC, 512> qg((int)g.lq.l, g.d, (two * 2 + values) * 64 + lane);
     float sv = 0.f;
     auto load = [&](const int e) {
         const int h = hk * g.group + e / per_head, r0 = (t0 + e % per_head) * 32;
@@ -232,23 +237,22 @@ __global__ __launch_bounds__(256, DT <= 64 ? 2 : 1) void sdpa_window_dkv_f32(con
     };
     if (from < to) load(from);
 
-    Frag kf[DT / 16], vf[DT / 16];
+    Frag mine[DT / 16];                                    // the key rows, or the value rows
     const long long el = b * g.lk.b + hk * g.lk.h + key * g.lk.l;
-    auto key_row = [&](const float *x) {
-        return [=](const int c) { return key < len ? load4(x + el, c, g.d, VEC) : f32x4{0.f, 0.f, 0.f, 0.f}; };
-    };
-    const float unk = pow2(-row_operand<DT>(kf, key_row(k), 1.0f, 1.0f)), unv = pow2(-row_operand<DT>(vf, key_row(v), 1.0f, 1.0f));
+    const float *mrow = (values ? v : k) + el;
+    const float unscale = pow2(-row_operand<DT>(mine, [&](const int c) { return key < len ? load4(mrow, c, g.d, VEC) : f32x4{0.f, 0.f, 0.f, 0.f}; }, 1.0f, 1.0f));
 
-    f32x16 dka[DT / 32], dva[DT / 32];
+    f32x16 acc[DT / 32];
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { dka[t][r] = 0.f; dva[t][r] = 0.f; }
+        for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     // The operands are 2^13 w, times a power of two where a column's weights are all tiny, and w (dP - delta) factor.
-    ColumnScale wscale, scale;
-    float wfactor = 1.0f, factor = 1.0f / 8192;
+    ColumnScale scale;
+    float factor = values ? 1.0f / 8192 : 1.0f;
     bool plain = false;                                    // every column has met a weight that needs no power
-    int nq = -63, ng = -63;                                // dka, dva are in units of 2^nq, 2^ng
+    int unit_power = -63;                                  // acc is in units of 2^unit_power
+    const u16 *first = values ? Gs : Qs, *then = values ? Qc : Gc;
 
     for (int e = from; e < to; ++e) {
         __syncthreads();
@@ -258,85 +262,93 @@ __global__ __launch_bounds__(256, DT <= 64 ? 2 : 1) void sdpa_window_dkv_f32(con
         if (e + 1 < to) load(e + 1);
         const int q0 = (t0 + e % per_head) * 32;
         const int p0 = g.w.q_offset + q0, p1 = g.w.q_offset + min(q0 + 31, g.Lq - 1);
-        if (tile_hidden(g.w, p0, p1, k0, len)) continue;
-        f32x16 s, dp;
+        const bool hidden = tile_hidden(g.w, p0, p1, k0, len), open = tile_open(g.w, p0, p1, k0, len) && q0 + 32 <= g.Lq;
+        f32x16 s;
+        if (!hidden) {
+            f32x16 s1;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+            for (int r = 0; r < 16; ++r) { s[r] = 0.f; s1[r] = 0.f; }
 #pragma unroll
-        for (int st = 0; st < DT / 16; ++st)
-            mma3x2(s, T::rows_frag(Qs, 0, st), kf[st], dp, T::rows_frag(Gs, 0, st), vf[st]);
-        const Powers qn(powers[0]), gn(powers[1]);
-        settle(s, dp);
+            for (int st = 0; st < DT / 16; st += 2)
+                mma3x2(s, T::rows_frag(first, 0, st), mine[st], s1, T::rows_frag(first, 0, st + 1), mine[st + 1]);
+            const i32x4 n = *reinterpret_cast<const i32x4 *>(powers[values]);
+            settle(s, s1);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const f32x4 m = *reinterpret_cast<const f32x4 *>(rowv + 8 * x + 4 * half), inv = *reinterpret_cast<const f32x4 *>(rowv + 32 + 8 * x + 4 * half),
-                        del = *reinterpret_cast<const f32x4 *>(rowv + 64 + 8 * x + 4 * half);
-            const float f = __builtin_ldexpf(unk, qn.n[x]), fp = __builtin_ldexpf(unv, gn.n[x]);
+            for (int x = 0; x < 4; ++x) {
+                const float f = __builtin_ldexpf(unscale, n[x]);
+                const f32x4 m = *reinterpret_cast<const f32x4 *>(rowv + (values ? 64 : 0) + 8 * x + 4 * half);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const int r = 4 * x + y;
-                s[r] = exp2_fast(__builtin_fmaf(s[r], f, -m[y])) * inv[y];
-                dp[r] = (s[r] * __builtin_fmaf(dp[r], fp, -del[y])) * factor;
+                for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_fmaf(s[4 * x + y] + s1[4 * x + y], f, -m[y]);     // s - m, or dP - delta
+            }
+            if (!values) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const f32x4 inv = *reinterpret_cast<const f32x4 *>(rowv + 32 + 8 * x + 4 * half);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) s[4 * x + y] = exp2_fast(s[4 * x + y]) * inv[y];
+                }
+                if (!open) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = q0 + acc_row(r) + 4 * half;
+                        s[r] = ((i < g.Lq) & sees(g.w, g.w.q_offset + i, key, len)) ? s[r] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) weights[(two * 4 + x) * 64 + lane] = f32x4{s[4 * x], s[4 * x + 1], s[4 * x + 2], s[4 * x + 3]};
             }
         }
-        if (!(tile_open(g.w, p0, p1, k0, len) && q0 + 32 <= g.Lq)) {
+        __syncthreads();
+        if (hidden) continue;
+        if (values) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = q0 + acc_row(r) + 4 * half;
-                const bool see = (i < g.Lq) & sees(g.w, g.w.q_offset + i, key, len);
-                s[r] = see ? s[r] : 0.f;
-                dp[r] = see ? dp[r] : 0.f;
+            for (int x = 0; x < 4; ++x) {
+                const f32x4 w = weights[(two * 4 + x) * 64 + lane];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const float ds = (w[y] * s[4 * x + y]) * factor;
+                    s[4 * x + y] = w[y] == 0.f ? 0.f : ds;               // (whatever stands in a query's rows that does not see the key)
+                }
             }
         }
-        if (!plain) {
-            s *= wfactor;
+        const Powers pw(powers[!values]);
+        if (pw.lo != unit_power || pw.hi != unit_power) {
+            const float unit = to_one_unit(pw, unit_power, s);
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
+        }
+        if (values || !plain) {
+            if (!values) s *= factor;
             float shrink;
-            if (wscale.fit_tiny(s, wfactor, shrink)) {
+            if (values ? scale.fit(s, factor, shrink) : scale.fit_tiny(s, factor, shrink)) {
 #pragma unroll
-                for (int t = 0; t < DT / 32; ++t) dva[t] *= shrink;
+                for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
             }
-            plain = !__any(wscale.fresh || wscale.c != 0);
-        }
-        if (qn.lo != nq || qn.hi != nq) {
-            const float unit = to_one_unit(qn, nq, dp);
-#pragma unroll
-            for (int t = 0; t < DT / 32; ++t) dka[t] *= unit;
-        }
-        if (gn.lo != ng || gn.hi != ng) {
-            const float unit = to_one_unit(gn, ng, s);
-#pragma unroll
-            for (int t = 0; t < DT / 32; ++t) dva[t] *= unit;
-        }
-        float shrink;
-        if (scale.fit(dp, factor, shrink)) {
-#pragma unroll
-            for (int t = 0; t < DT / 32; ++t) dka[t] *= shrink;
+            plain = !__any(scale.fresh || scale.c != 0);
         }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            const Frag wf = acc_frag(s, st), df = acc_frag(dp, st);
+            const Frag f = acc_frag(s, st);
+            Frag c[DT / 32];
 #pragma unroll
-            for (int t = 0; t < DT / 32; ++t) mma3x2(dva[t], T::cols_frag(Gc, t, st), wf, dka[t], T::cols_frag(Qc, t, st), df);
+            for (int t = 0; t < DT / 32; ++t) c[t] = T::cols_frag(then, t, st);
+            mma3(acc, c, f);
         }
     }
 
 #pragma unroll
-    for (int t = 0; t < DT / 32; ++t) settle(dka[t], dva[t]);
+    for (int t = 0; t < DT / 32; ++t) settle(acc[t]);
     if (key >= g.Lk) return;
     // q was staged as q rT log2(e): dk = rT sum dS q = ln(2) of what was summed
-    constexpr float LN2 = 0.69314718055994530942f;
-    const bool whole = kb.chunks[cl] == 1;
-    float *part = whole ? nullptr : partial_sums(kb, pair, block, chunk, g.d) + (wave * 32 + ln) * (long long)g.d;
-    float *ok = whole ? dk + el : part, *ov = whole ? dv + el : part + 128ll * g.d;
-    const float k0f = pow2(-scale.c), k1f = pow2(nq), vf0 = pow2(-13 - wscale.c), vf1 = pow2(ng);
+    const float f0 = pow2((values ? 0 : -13) - scale.c) * (values ? 0.69314718055994530942f : 1.0f), f1 = pow2(unit_power);
+    float *to_row = (values ? dk : dv) + el;
+    if (kb.chunks[cl] > 1) to_row = partial_sums(kb, pair, block, chunk, g.d) + (values ? 0 : 128ll * g.d) + (two * 32 + ln) * (long long)g.d;
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            f32x4 x = {dka[t][4 * r], dka[t][4 * r + 1], dka[t][4 * r + 2], dka[t][4 * r + 3]};
-            f32x4 y = {dva[t][4 * r], dva[t][4 * r + 1], dva[t][4 * r + 2], dva[t][4 * r + 3]};
-            store4(ok, 32 * t + 8 * r + 4 * half, g.d, VEC, ((x * k0f) * k1f) * LN2);
-            store4(ov, 32 * t + 8 * r + 4 * half, g.d, VEC, (y * vf0) * vf1);
+            f32x4 x = {acc[t][4 * r], acc[t][4 * r + 1], acc[t][4 * r + 2], acc[t][4 * r + 3]};
+            store4(to_row, 32 * t + 8 * r + 4 * half, g.d, VEC, (x * f0) * f1);
         }
 }
 

@@ -299,31 +299,33 @@ struct Tile {
     }
 };
 
-// Two R x C tiles (A, B) staged together by 256 threads: a thread loads 4 x 4 pieces, splits them and writes them in row form
+// Two R x C tiles (A, B) staged together by NT threads: a thread loads 4 x 4 pieces, splits them and writes them in row form
 // and / or, exchanged pairwise, in column form.  The pieces that a wavefront handles at a time are whole rows of one tile
 // (C is rounded up to a power of two for that), so it finds their largest value and their power of two by itself; the
 // powers go to LDS with the tile, one for every eight rows.
-template <int R, int C, bool VEC>
+template <int R, int C, bool VEC, int NT = 256>
 struct Stage {
     typedef Tile<R, C> T;
     static constexpr int GROUPS = (C <= 32 ? 32 : (C <= 64 ? 64 : 128)) / 4;      // of four columns
-    static constexpr int QUADS = (R / 4) * GROUPS, NP = (2 * QUADS + 255) / 256, WAVE_ROWS = 256 / GROUPS;
+    static constexpr int QUADS = (R / 4) * GROUPS, NP = (2 * QUADS + NT - 1) / NT, WAVE_ROWS = 256 / GROUPS;
     static_assert(QUADS % 64 == 0 && WAVE_ROWS >= 8, "pieces");
     f32x4 x[NP][4];
     unsigned from[NP];       // byte offset of the thread's piece in its tensor's tile
     int to_row[NP], to_col[NP];
     int run[2] = {63, 63};   // smallest power so far of the rows this wavefront stages of either tile
 
-    __device__ static __forceinline__ int piece(const int i) { return threadIdx.x + 256 * i; }
-    __device__ static __forceinline__ bool has(const int i) { return 256 * i + 256 <= 2 * QUADS || __builtin_amdgcn_readfirstlane(piece(i)) < 2 * QUADS; }
-    __device__ static __forceinline__ bool second(const int i) {
-        return QUADS % 256 == 0 ? 256 * i >= QUADS : __builtin_amdgcn_readfirstlane(piece(i)) >= QUADS;
-    }
-    __device__ static __forceinline__ int row(const int i) { return (piece(i) - second(i) * QUADS) / GROUPS * 4; }
-    __device__ static __forceinline__ int col(const int i) { return piece(i) % GROUPS * 4; }
-    __device__ static __forceinline__ bool inside(const int i) { return C == 4 * GROUPS || col(i) < C; }
+    const int tid;           // the thread's number in the order in which wavefronts are given pieces
 
-    __device__ __forceinline__ Stage(const int stride, const int d) {
+    __device__ __forceinline__ int piece(const int i) const { return tid + NT * i; }
+    __device__ __forceinline__ bool has(const int i) const { return NT * (i + 1) <= 2 * QUADS || __builtin_amdgcn_readfirstlane(piece(i)) < 2 * QUADS; }
+    __device__ __forceinline__ bool second(const int i) const {
+        return QUADS % NT == 0 ? NT * i >= QUADS : __builtin_amdgcn_readfirstlane(piece(i)) >= QUADS;
+    }
+    __device__ __forceinline__ int row(const int i) const { return (piece(i) - second(i) * QUADS) / GROUPS * 4; }
+    __device__ __forceinline__ int col(const int i) const { return piece(i) % GROUPS * 4; }
+    __device__ __forceinline__ bool inside(const int i) const { return C == 4 * GROUPS || col(i) < C; }
+
+    __device__ __forceinline__ Stage(const int stride, const int d, const int thread) : tid(thread) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             from[i] = col(i) < d ? (unsigned)(row(i) * stride + col(i)) * 4u : NOWHERE;
@@ -366,7 +368,7 @@ struct Stage {
             float m = wave_max_abs(largest(x[i]));
             if (__builtin_expect(m == INFINITY, 0)) m = wave_max_abs(largest_finite(x[i]));
             if (SCALED && !b) m *= fabsf(f0 * f1);
-            int &least = QUADS % 256 == 0 ? run[b] : run[0];       // (a wavefront has either pieces of one tile only, or these in turn)
+            int &least = QUADS % NT == 0 ? run[b] : run[0];       // (a wavefront has either pieces of one tile only, or these in turn)
             const int a = least = min(least, coarse_scale_of(m)), lane = threadIdx.x & 63;
             if (lane < WAVE_ROWS / 8) powers[(b ? R / 8 : 0) + (__builtin_amdgcn_readfirstlane(row(i)) >> 3) + lane] = -a;
             if (b) put<ROWS_B, COLS_B, false>(i, rows_b, cols_b, pow2(a), f0, f1);

@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
 
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;      // keys between them no query here sees
-    Stage<BN, DT, VEC> kv(ks, g.d);
+    Stage<BN, DT, VEC> kv(ks, g.d, threadIdx.x);
     auto load = [&](const int i) { kv.load(kp, vp, ks, at.key0(i), min(at.len, at.wp1 + 1), g.d, hide0, hide1); };
     if (at.tiles > 0) load(0);
 
