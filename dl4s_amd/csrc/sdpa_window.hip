@@ -288,7 +288,7 @@ template <int DT, bool VEC>
 int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats, const float *dout,
                float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
     typedef Tile<32, DT> T;
-    const size_t lds_q = 2 * 2 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 4 * (T::ROWS_PLANE + T::COLS_PLANE) + 16384;
+    const size_t lds_q = 2 * 2 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 2 * 4 * (T::ROWS_PLANE + T::COLS_PLANE) + 16384;
     int rc = lds_limit(ctx, dl4s::LDS_WINDOW, 2 * (DT / 32 - 1) + VEC, sdpa_window_dq_f32<DT, VEC>, lds_q);
     if (!rc) rc = lds_limit(ctx, dl4s::LDS_WINDOW_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dkv_f32<DT, VEC>, lds_k);
     if (rc) return rc;

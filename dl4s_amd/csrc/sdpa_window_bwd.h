@@ -196,10 +196,10 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
                                                                const KeyBlocks kb) {
     typedef Tile<32, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
-    u16 *Qs = window_lds, *Gs = Qs + 2 * T::ROWS_PLANE, *Qc = Gs + 2 * T::ROWS_PLANE, *Gc = Qc + 2 * T::COLS_PLANE;
-    f32x4 *weights = reinterpret_cast<f32x4 *>(Gc + 2 * T::COLS_PLANE);        // [pair of wavefronts][4][lane]
-    __shared__ __align__(16) float rowv[96];               // [3][32]: m, 2^13 / l, delta of the tile's queries
-    __shared__ __align__(16) int powers[2][4];             // [Q, dO]
+    constexpr int BUF = 4 * (T::ROWS_PLANE + T::COLS_PLANE);     // [Q rows][dO rows][Q columns][dO columns]
+    f32x4 *weights = reinterpret_cast<f32x4 *>(window_lds + 2 * BUF);      // [pair of wavefronts][4][lane]
+    __shared__ __align__(16) float row_values[2][96];      // [buffer][3][32]: m, 2^13 / l, delta of the tile's queries
+    __shared__ __align__(16) int powers[2][2][4];          // [buffer][Q, dO]
 
     int id = blockIdx.x, cl = 1;
     if (id >= 8 * kb.per_xcd[1]) { id -= 8 * kb.per_xcd[1]; cl = 0; }
@@ -235,6 +235,13 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
             if (which == 1) sv *= 8192.0f;
         }
     };
+    auto stage = [&](const int e) {
+        const int buf = (e - from) & 1;
+        u16 *Qs = window_lds + buf * BUF, *Gs = Qs + 2 * T::ROWS_PLANE, *Qc = Gs + 2 * T::ROWS_PLANE, *Gc = Qc + 2 * T::COLS_PLANE;
+        qg.template store<true, true, true, true, true>(Qs, Qc, Gs, Gc, &powers[buf][0][0], g.rT, LOG2E);
+        if (threadIdx.x < 96) row_values[buf][threadIdx.x] = sv;
+        if (e + 1 < to) load(e + 1);
+    };
     if (from < to) load(from);
 
     Frag mine[DT / 16];                                    // the key rows, or the value rows
@@ -252,14 +259,18 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
     float factor = values ? 1.0f / 8192 : 1.0f;
     bool plain = false;                                    // every column has met a weight that needs no power
     int unit_power = -63;                                  // acc is in units of 2^unit_power
-    const u16 *first = values ? Gs : Qs, *then = values ? Qc : Gc;
 
+    // Two buffers: behind the exchange of the weights one wavefront of a pair multiplies and then stages its share of the next
+    // tile, the other stages first, so that on their SIMD one's vector work runs beside the other's matrix instructions.
+    if (from < to) {
+        stage(from);
+        __syncthreads();
+    }
     for (int e = from; e < to; ++e) {
-        __syncthreads();
-        qg.template store<true, true, true, true, true>(Qs, Qc, Gs, Gc, &powers[0][0], g.rT, LOG2E);
-        if (threadIdx.x < 96) rowv[threadIdx.x] = sv;
-        __syncthreads();
-        if (e + 1 < to) load(e + 1);
+        const int buf = (e - from) & 1;
+        const u16 *rows_at = window_lds + buf * BUF, *cols_at = rows_at + 4 * T::ROWS_PLANE;
+        const u16 *first = rows_at + (values ? 2 * T::ROWS_PLANE : 0), *then = cols_at + (values ? 0 : 2 * T::COLS_PLANE);
+        const float *rowv = row_values[buf];
         const int q0 = (t0 + e % per_head) * 32;
         const int p0 = g.w.q_offset + q0, p1 = g.w.q_offset + min(q0 + 31, g.Lq - 1);
         const bool hidden = tile_hidden(g.w, p0, p1, k0, len), open = tile_open(g.w, p0, p1, k0, len) && q0 + 32 <= g.Lq;
@@ -271,7 +282,7 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
 #pragma unroll
             for (int st = 0; st < DT / 16; st += 2)
                 mma3x2(s, T::rows_frag(first, 0, st), mine[st], s1, T::rows_frag(first, 0, st + 1), mine[st + 1]);
-            const i32x4 n = *reinterpret_cast<const i32x4 *>(powers[values]);
+            const i32x4 n = *reinterpret_cast<const i32x4 *>(powers[buf][values]);
             settle(s, s1);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -299,41 +310,45 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
             }
         }
         __syncthreads();
-        if (hidden) continue;
-        if (values) {
+        if (!values && e + 1 < to) stage(e + 1);
+        if (!hidden) {
+            if (values) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const f32x4 w = weights[(two * 4 + x) * 64 + lane];
+                for (int x = 0; x < 4; ++x) {
+                    const f32x4 w = weights[(two * 4 + x) * 64 + lane];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const float ds = (w[y] * s[4 * x + y]) * factor;
-                    s[4 * x + y] = w[y] == 0.f ? 0.f : ds;               // (whatever stands in a query's rows that does not see the key)
+                    for (int y = 0; y < 4; ++y) {
+                        const float ds = (w[y] * s[4 * x + y]) * factor;
+                        s[4 * x + y] = w[y] == 0.f ? 0.f : ds;           // (whatever stands in a query's rows that does not see the key)
+                    }
                 }
             }
-        }
-        const Powers pw(powers[!values]);
-        if (pw.lo != unit_power || pw.hi != unit_power) {
-            const float unit = to_one_unit(pw, unit_power, s);
+            const Powers pw(powers[buf][!values]);
+            if (pw.lo != unit_power || pw.hi != unit_power) {
+                const float unit = to_one_unit(pw, unit_power, s);
 #pragma unroll
-            for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
-        }
-        if (values || !plain) {
-            if (!values) s *= factor;
-            float shrink;
-            if (values ? scale.fit(s, factor, shrink) : scale.fit_tiny(s, factor, shrink)) {
-#pragma unroll
-                for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
+                for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
             }
-            plain = !__any(scale.fresh || scale.c != 0);
-        }
+            if (values || !plain) {
+                if (!values) s *= factor;
+                float shrink;
+                if (values ? scale.fit(s, factor, shrink) : scale.fit_tiny(s, factor, shrink)) {
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-            const Frag f = acc_frag(s, st);
-            Frag c[DT / 32];
+                    for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
+                }
+                plain = !__any(scale.fresh || scale.c != 0);
+            }
 #pragma unroll
-            for (int t = 0; t < DT / 32; ++t) c[t] = T::cols_frag(then, t, st);
-            mma3(acc, c, f);
+            for (int st = 0; st < 2; ++st) {
+                const Frag f = acc_frag(s, st);
+                Frag c[DT / 32];
+#pragma unroll
+                for (int t = 0; t < DT / 32; ++t) c[t] = T::cols_frag(then, t, st);
+                mma3(acc, c, f);
+            }
         }
+        if (values && e + 1 < to) stage(e + 1);
+        __syncthreads();
     }
 
 #pragma unroll
