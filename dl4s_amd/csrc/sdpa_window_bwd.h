@@ -7,7 +7,7 @@
 //     group.  Two wavefronts share 32 keys (the columns of their accumulators): one holds K and forms S = Q . K^T, the weights
 //     w, and dV^T += dO^T . w, the other holds V and forms dP = dO . V^T and, with the weights it gets through LDS,
 //     dK^T += Q^T . dS.  That halves what a wavefront keeps in registers, so two run on a SIMD at every head dim (one
-//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes DKV_US at B2 H16/4 L4096 d96 window 777).
+//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes 427 us at B2 H16/4 L4096 d96 window 777).
 //     Shared key heads are summed in the accumulators, in a fixed order, without atomics.  Key blocks that hold visible
 //     first keys are seen by every later query: their query tiles are dealt to several workgroups whose partial sums a
 //     last kernel adds up in order; so are all blocks where that shortens the longest queue of a compute unit.
@@ -79,19 +79,23 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;
     Stage<32, DT, VEC> kv(ks, g.d, threadIdx.x);
-    auto load = [&](const int i) { kv.load(kp, vp, ks, at.key0(i), min(at.len, at.wp1 + 1), g.d, hide0, hide1); };
+    const int keys = min(at.len, at.wp1 + 1);
+    auto load = [&](const int i) {
+        const int k0 = at.key0(i);
+        kv.load(kp + (long long)k0 * ks, vp + (long long)k0 * ks, ks, k0, keys - k0, g.d, hide0, hide1);
+    };
     if (at.tiles > 0) load(0);
 
     const long long el = at.b * g.lq.b + at.h * g.lq.h + at.qc * g.lq.l, row = ((long long)at.b * g.H + at.h) * g.Lq + at.qc;
     Frag qf[DT / 16], gf[DT / 16];
-    const float unq = pow2(-row_operand<DT>(qf, [&](const int c) { return load4(q + el, c, g.d, VEC); }, g.rT, LOG2E));
+    const float unq = pow2(-row_operand<DT>(qf, [&](const int c) { return load4(q + el, c, g.d, VEC); }, g.rT * LOG2E));
     float del = 0.f;
     const float ung = pow2(-row_operand<DT>(gf, [&](const int c) {
         const f32x4 x = load4(dout + el, c, g.d, VEC), o = load4(out + el, c, g.d, VEC);
 #pragma unroll
         for (int e = 0; e < 4; ++e) del += x[e] * o[e];
         return x;
-    }, 1.0f, 1.0f));
+    }, 1.0f));
     del = sum_halves(del);
     const float m = stats[2 * row], inv = stats[2 * row + 1];
     if (half == 0 && at.qi < g.Lq) delta[row] = del;
@@ -109,7 +113,7 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
-        kv.template store<true, true, true, false, false>(Ks, Kc, Vs, nullptr, &powers[0][0]);
+        kv.template store<true, true, true, false>(Ks, Kc, Vs, nullptr, &powers[0][0]);
         __syncthreads();
         if (i + 1 < at.tiles) load(i + 1);
         const int k0 = at.key0(i);
@@ -225,29 +229,44 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
     // (wavefronts take pieces of the tiles in the order 0, 4, 1, 5, ...: where there are fewer pieces, both kinds get some)
     Stage<32, DT, VEC, 512> qg((int)g.lq.l, g.d, (two * 2 + values) * 64 + lane);
     float sv = 0.f;
-    auto load = [&](const int e) {
-        const int h = hk * g.group + e / per_head, r0 = (t0 + e % per_head) * 32;
-        qg.load(q + b * g.lq.b + h * g.lq.h, dout + b * g.lq.b + h * g.lq.h, (int)g.lq.l, r0, rows, g.d);
+    // the next tile to be loaded: its place, and where it lies
+    int next = t0 + (per_head ? from % per_head : 0);
+    const int head0 = hk * g.group + (per_head ? from / per_head : 0), qs = (int)g.lq.l;
+    const float *qp = q + b * g.lq.b + head0 * g.lq.h + (long long)next * 32 * qs, *gp = dout + (qp - q);
+    long long row0 = ((long long)b * g.H + head0) * g.Lq;
+    auto load = [&]() {
+        const int r0 = next * 32;
+        qg.load(qp, gp, qs, r0, rows - r0, g.d);
         if (threadIdx.x < 96) {
             const int which = threadIdx.x >> 5, r = r0 + (threadIdx.x & 31);
-            const long long row = ((long long)b * g.H + h) * g.Lq + r;
-            sv = r < rows ? (which == 2 ? delta[row] : stats[2 * row + which]) : 0.f;
+            sv = 0.f;
+            if (r < rows) sv = which == 2 ? delta[row0 + r] : stats[2 * (row0 + r) + which];
             if (which == 1) sv *= 8192.0f;
+        }
+        if (++next == t1) {                                // on to the group's next head
+            next = t0;
+            qp += g.lq.h - (long long)(t1 - 1 - t0) * 32 * qs;
+            gp += g.lq.h - (long long)(t1 - 1 - t0) * 32 * qs;
+            row0 += g.Lq;
+        } else {
+            qp += 32 * qs;
+            gp += 32 * qs;
         }
     };
     auto stage = [&](const int e) {
         const int buf = (e - from) & 1;
         u16 *Qs = window_lds + buf * BUF, *Gs = Qs + 2 * T::ROWS_PLANE, *Qc = Gs + 2 * T::ROWS_PLANE, *Gc = Qc + 2 * T::COLS_PLANE;
-        qg.template store<true, true, true, true, true>(Qs, Qc, Gs, Gc, &powers[buf][0][0], g.rT, LOG2E);
+        qg.template store<true, true, true, true>(Qs, Qc, Gs, Gc, &powers[buf][0][0], g.rT * LOG2E);
         if (threadIdx.x < 96) row_values[buf][threadIdx.x] = sv;
-        if (e + 1 < to) load(e + 1);
+        if (e + 1 < to) load();
     };
-    if (from < to) load(from);
+    int now = next;                                        // the tile that is worked on
+    if (from < to) load();
 
     Frag mine[DT / 16];                                    // the key rows, or the value rows
     const long long el = b * g.lk.b + hk * g.lk.h + key * g.lk.l;
     const float *mrow = (values ? v : k) + el;
-    const float unscale = pow2(-row_operand<DT>(mine, [&](const int c) { return key < len ? load4(mrow, c, g.d, VEC) : f32x4{0.f, 0.f, 0.f, 0.f}; }, 1.0f, 1.0f));
+    const float unscale = pow2(-row_operand<DT>(mine, [&](const int c) { return key < len ? load4(mrow, c, g.d, VEC) : f32x4{0.f, 0.f, 0.f, 0.f}; }, 1.0f));
 
     f32x16 acc[DT / 32];
 #pragma unroll
@@ -271,25 +290,24 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
         const u16 *rows_at = window_lds + buf * BUF, *cols_at = rows_at + 4 * T::ROWS_PLANE;
         const u16 *first = rows_at + (values ? 2 * T::ROWS_PLANE : 0), *then = cols_at + (values ? 0 : 2 * T::COLS_PLANE);
         const float *rowv = row_values[buf];
-        const int q0 = (t0 + e % per_head) * 32;
+        const int q0 = now * 32;
+        now = now + 1 == t1 ? t0 : now + 1;
         const int p0 = g.w.q_offset + q0, p1 = g.w.q_offset + min(q0 + 31, g.Lq - 1);
         const bool hidden = tile_hidden(g.w, p0, p1, k0, len), open = tile_open(g.w, p0, p1, k0, len) && q0 + 32 <= g.Lq;
         f32x16 s;
         if (!hidden) {
-            f32x16 s1;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { s[r] = 0.f; s1[r] = 0.f; }
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-            for (int st = 0; st < DT / 16; st += 2)
-                mma3x2(s, T::rows_frag(first, 0, st), mine[st], s1, T::rows_frag(first, 0, st + 1), mine[st + 1]);
+            for (int st = 0; st < DT / 16; ++st) s = mma3(T::rows_frag(first, 0, st), mine[st], s);
             const i32x4 n = *reinterpret_cast<const i32x4 *>(powers[buf][values]);
-            settle(s, s1);
+            settle(s);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const float f = __builtin_ldexpf(unscale, n[x]);
                 const f32x4 m = *reinterpret_cast<const f32x4 *>(rowv + (values ? 64 : 0) + 8 * x + 4 * half);
 #pragma unroll
-                for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_fmaf(s[4 * x + y] + s1[4 * x + y], f, -m[y]);     // s - m, or dP - delta
+                for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_fmaf(s[4 * x + y], f, -m[y]);     // s - m, or dP - delta
             }
             if (!values) {
 #pragma unroll

@@ -145,7 +145,7 @@ struct Planes {
 __device__ __forceinline__ unsigned round2(const float a, const float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
-// The planes of four values times a power of two s.
+// The planes of four values times s.
 __device__ __forceinline__ void split4(const f32x4 v, const float s, Planes &p, Planes &q) {
     asm("v_fma_mixlo_f16 %0, %4, %8, 0\n\t"
         "v_fma_mixhi_f16 %0, %5, %8, 0\n\t"
@@ -223,10 +223,11 @@ __device__ __forceinline__ f32x2 both_halves(const float v) {
 __device__ __forceinline__ float max_halves(const float v) { const f32x2 r = both_halves(v); return fmaxf(r.x, r.y); }
 __device__ __forceinline__ float sum_halves(const float v) { const f32x2 r = both_halves(v); return r.x + r.y; }
 
-// A row of up to DT columns, one row per lane of a half wavefront (lane and lane ^ 32 share it), as the operand whose
-// contraction runs along the row; f0 and f1 are multiplied in one after the other.  Returns the row's power of two.
+// A row of up to DT columns times a factor, one row per lane of a half wavefront (lane and lane ^ 32 share it), as the operand
+// whose contraction runs along the row.  The factor goes into the splitting: a plane is rounded from the exact product.
+// Returns the row's power of two.
 template <int DT, typename Load>
-__device__ __forceinline__ int row_operand(Frag (&f)[DT / 16], const Load load, const float f0, const float f1) {
+__device__ __forceinline__ int row_operand(Frag (&f)[DT / 16], const Load load, const float factor) {
     const int half = (threadIdx.x & 63) >> 5;
     f32x4 x[DT / 8];
 #pragma unroll
@@ -234,14 +235,10 @@ __device__ __forceinline__ int row_operand(Frag (&f)[DT / 16], const Load load, 
         x[2 * s] = load(16 * s + 8 * half);
         x[2 * s + 1] = load(16 * s + 8 * half + 4);
     }
-#pragma unroll
-    for (int i = 0; i < DT / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][e] = (x[i][e] * f0) * f1;
     float top = max_halves(largest(x));
     if (__any(top == INFINITY)) top = max_halves(largest_finite(x));
-    const int a = scale_of(top);
-    const float p = pow2(a);
+    const int a = scale_of(top * fabsf(factor));
+    const float p = pow2(a) * factor;
 #pragma unroll
     for (int s = 0; s < DT / 16; ++s) {
         Planes w[4];
@@ -252,13 +249,11 @@ __device__ __forceinline__ int row_operand(Frag (&f)[DT / 16], const Load load, 
     return a;
 }
 
-// Rows of a tile of fp32 tensors through a buffer descriptor made per tile: rows at or beyond the tensor's valid ones, and
-// columns at or beyond d (whose offset lies outside every descriptor), read as zeros without a branch.
+// Rows of a tile of an fp32 tensor through a buffer descriptor made per tile (base: the tile's first row): rows from `rows` on,
+// and columns at or beyond d (whose offset lies outside every descriptor), read as zeros without a branch.
 constexpr unsigned NOWHERE = 0x80000000u;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const float *base, const int stride, const int r0, const int rows, const int n,
-                                                            const int d) {
-    const int m = min(rows - r0, n);
-    return __builtin_amdgcn_make_buffer_rsrc((void *)(base + (long long)r0 * stride), 0, m > 0 ? ((m - 1) * stride + d) * 4 : 0, 0x00020000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const float *base, const int stride, const int rows, const int d) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, rows > 0 ? ((rows - 1) * stride + d) * 4 : 0, 0x00020000);
 }
 // at: byte offset of the piece's first column, NOWHERE (or above) where the piece lies outside; left: columns from it to d
 template <bool VEC>
@@ -314,18 +309,17 @@ struct Stage {
     int to_row[NP], to_col[NP];
     int run[2] = {63, 63};   // smallest power so far of the rows this wavefront stages of either tile
 
-    const int tid;           // the thread's number in the order in which wavefronts are given pieces
+    const int tid, wave0;    // the thread's number, and its wavefront's first, in the order in which wavefronts are given pieces
 
     __device__ __forceinline__ int piece(const int i) const { return tid + NT * i; }
-    __device__ __forceinline__ bool has(const int i) const { return NT * (i + 1) <= 2 * QUADS || __builtin_amdgcn_readfirstlane(piece(i)) < 2 * QUADS; }
-    __device__ __forceinline__ bool second(const int i) const {
-        return QUADS % NT == 0 ? NT * i >= QUADS : __builtin_amdgcn_readfirstlane(piece(i)) >= QUADS;
-    }
+    __device__ __forceinline__ bool has(const int i) const { return NT * (i + 1) <= 2 * QUADS || wave0 + NT * i < 2 * QUADS; }
+    __device__ __forceinline__ bool second(const int i) const { return QUADS % NT == 0 ? NT * i >= QUADS : wave0 + NT * i >= QUADS; }
     __device__ __forceinline__ int row(const int i) const { return (piece(i) - second(i) * QUADS) / GROUPS * 4; }
     __device__ __forceinline__ int col(const int i) const { return piece(i) % GROUPS * 4; }
     __device__ __forceinline__ bool inside(const int i) const { return C == 4 * GROUPS || col(i) < C; }
 
-    __device__ __forceinline__ Stage(const int stride, const int d, const int thread) : tid(thread) {
+    __device__ __forceinline__ Stage(const int stride, const int d, const int thread)
+        : tid(thread), wave0(__builtin_amdgcn_readfirstlane(thread)) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             from[i] = col(i) < d ? (unsigned)(row(i) * stride + col(i)) * 4u : NOWHERE;
@@ -336,10 +330,11 @@ struct Stage {
             to_col[i] = col(i) * R + ((at ^ T::swap(col(i))) << 3) + sub;
         }
     }
-    // rows [r0, r0 + R) of both tensors, of which those below `rows` are valid; rows [hide0, hide1) are taken as zeros
+    // a, b: row r0 of either tensor; of its next R rows `rows` are valid, and those that are [hide0, hide1) of the tensor are taken
+    // as zeros
     __device__ __forceinline__ void load(const float *a, const float *b, const int stride, const int r0, const int rows, const int d,
                                          const int hide0 = 0, const int hide1 = 0) {
-        const __amdgpu_buffer_rsrc_t ra = tile_rows(a, stride, r0, rows, R, d), rb = tile_rows(b, stride, r0, rows, R, d);
+        const __amdgpu_buffer_rsrc_t ra = tile_rows(a, stride, min(rows, R), d), rb = tile_rows(b, stride, min(rows, R), d);
         const bool cut = r0 < hide1 && r0 + R > hide0;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
@@ -357,33 +352,31 @@ struct Stage {
             for (int j = 0; j < 4; ++j) x[i][j] = tile_load4<VEC>(second(i) ? rb : ra, at[j], VEC ? 0 : d - col(i));
         }
     }
-    // f0, f1: factors of tile A's values, multiplied in one after the other (where SCALED).  powers: [A, B][R / 8], negated.
-    template <bool ROWS_A, bool COLS_A, bool ROWS_B, bool COLS_B, bool SCALED>
-    __device__ __forceinline__ void store(u16 *rows_a, u16 *cols_a, u16 *rows_b, u16 *cols_b, int *powers, const float f0 = 1.0f,
-                                          const float f1 = 1.0f) {
+    // fa: a factor of tile A's values.  powers: [A, B][R / 8], negated.
+    template <bool ROWS_A, bool COLS_A, bool ROWS_B, bool COLS_B>
+    __device__ __forceinline__ void store(u16 *rows_a, u16 *cols_a, u16 *rows_b, u16 *cols_b, int *powers, const float fa = 1.0f) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             if (!has(i)) continue;
             const bool b = second(i);
             float m = wave_max_abs(largest(x[i]));
             if (__builtin_expect(m == INFINITY, 0)) m = wave_max_abs(largest_finite(x[i]));
-            if (SCALED && !b) m *= fabsf(f0 * f1);
+            const float f = b ? 1.0f : fa;
             int &least = QUADS % NT == 0 ? run[b] : run[0];       // (a wavefront has either pieces of one tile only, or these in turn)
-            const int a = least = min(least, coarse_scale_of(m)), lane = threadIdx.x & 63;
-            if (lane < WAVE_ROWS / 8) powers[(b ? R / 8 : 0) + (__builtin_amdgcn_readfirstlane(row(i)) >> 3) + lane] = -a;
-            if (b) put<ROWS_B, COLS_B, false>(i, rows_b, cols_b, pow2(a), f0, f1);
-            else put<ROWS_A, COLS_A, SCALED>(i, rows_a, cols_a, pow2(a), f0, f1);
+            const int a = least = min(least, coarse_scale_of(m * fabsf(f))), lane = threadIdx.x & 63;
+            if (lane < WAVE_ROWS / 8) powers[(b ? R / 8 : 0) + ((wave0 + NT * i - b * QUADS) / GROUPS >> 1) + lane] = -a;
+            if (b) put<ROWS_B, COLS_B>(i, rows_b, cols_b, pow2(a));
+            else put<ROWS_A, COLS_A>(i, rows_a, cols_a, pow2(a) * f);
         }
     }
-    template <bool ROWS, bool COLS, bool SCALED>
-    __device__ __forceinline__ void put(const int i, u16 *rows, u16 *cols, const float p2, const float f0, const float f1) const {
+    // scale: a power of two times the factor
+    template <bool ROWS, bool COLS>
+    __device__ __forceinline__ void put(const int i, u16 *rows, u16 *cols, const float scale) const {
         if (!inside(i)) return;
         Planes w[4][2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            f32x4 v = x[i][j];
-            if (SCALED) v = (v * f0) * f1;
-            split4(v, p2, w[j][0], w[j][1]);
+            split4(x[i][j], scale, w[j][0], w[j][1]);
             if (ROWS) {
                 u16 *tr = rows + to_row[i] + j * (C + 8);
                 *reinterpret_cast<u32x2 *>(tr) = u32x2{w[j][0].h, w[j][1].h};

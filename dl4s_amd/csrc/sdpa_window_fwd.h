@@ -76,13 +76,17 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;      // keys between them no query here sees
     Stage<BN, DT, VEC> kv(ks, g.d, threadIdx.x);
-    auto load = [&](const int i) { kv.load(kp, vp, ks, at.key0(i), min(at.len, at.wp1 + 1), g.d, hide0, hide1); };
+    const int keys = min(at.len, at.wp1 + 1);
+    auto load = [&](const int i) {
+        const int k0 = at.key0(i);
+        kv.load(kp + (long long)k0 * ks, vp + (long long)k0 * ks, ks, k0, keys - k0, g.d, hide0, hide1);
+    };
     if (at.tiles > 0) load(0);
 
     // scores in the base-2 exponent domain
     Frag qf[DT / 16];
     const float *qp = q + at.b * g.lq.b + at.h * g.lq.h + at.qc * g.lq.l;
-    const float unq = pow2(-row_operand<DT>(qf, [&](const int c) { return load4(qp, c, g.d, VEC); }, g.rT, LOG2E));
+    const float unq = pow2(-row_operand<DT>(qf, [&](const int c) { return load4(qp, c, g.d, VEC); }, g.rT * LOG2E));
     const int p0 = g.w.q_offset + at.q0, p1 = g.w.q_offset + min(at.q0 + 31, g.Lq - 1), p = g.w.q_offset + at.qi;
     const bool idle = at.q0 >= g.Lq;
 
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
-        kv.template store<true, false, false, true, false>(Ks, nullptr, nullptr, Vc, &powers[0][0]);
+        kv.template store<true, false, false, true>(Ks, nullptr, nullptr, Vc, &powers[0][0]);
         __syncthreads();
         if (i + 1 < at.tiles) load(i + 1);
         const int t0 = at.key0(i);
