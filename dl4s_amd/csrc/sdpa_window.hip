@@ -201,6 +201,11 @@ inline Layout layout(bool token_major, int64_t heads, int64_t L, int64_t d) {
     return token_major ? Layout{L * heads * d, d, heads * d} : Layout{heads * L * d, L * d, d};
 }
 inline dim3 row_grid(long long rows) { return dim3((unsigned)((rows + 3) / 4)); }
+// A launch has fewer than 2^32 threads along its first axis: refused before anything is launched.
+inline int fits_a_launch(const char *what, long long workgroups, int threads) {
+    DL4S_REQUIRE(workgroups < (1ll << 32) / threads, DL4S_HIP_EUNSUPPORTED, "%s: %lld workgroups of %d threads", what, workgroups, threads);
+    return DL4S_HIP_OK;
+}
 
 inline bool on_16_bytes(std::initializer_list<const void *> ps) {
     uintptr_t bits = 0;
@@ -324,8 +329,8 @@ int launch_bwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const fl
 template <int DT, int NW>
 int launch_few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, FewArgs &a, int64_t pairs) {
     const int most_cols = std::min(16, a.cols);
-    const size_t lds = (size_t)NW * most_cols * (DT + 4) * sizeof(float);
-    const int rc = lds_limit(ctx, dl4s::LDS_WINDOW_FEW, DT == 64 ? 0 : (DT == 128 ? 1 : 2), sdpa_window_few_f32<DT, NW>, lds);
+    const size_t of_row = (size_t)NW * (DT + 4) * sizeof(float), lds = most_cols * of_row;
+    const int rc = lds_limit(ctx, dl4s::LDS_WINDOW_FEW, DT == 64 ? 0 : (DT == 128 ? 1 : 2), sdpa_window_few_f32<DT, NW>, 16 * of_row);
     if (rc) return rc;
     hipLaunchKernelGGL((sdpa_window_few_f32<DT, NW>), dim3(a.nsplit, (unsigned)pairs, (a.cols + 15) / 16), dim3(NW * 64), lds, ctx->stream, q, k,
                        v, out, stats, a);
@@ -377,9 +382,9 @@ int window_checks(const char *what, int64_t B, int64_t H, int64_t Hkv, int64_t L
     DL4S_REQUIRE(H == 0 || (Hkv > 0 && H % Hkv == 0), DL4S_HIP_ESHAPE, "%s: %lld query heads do not share %lld key heads evenly", what,
                  (long long)H, (long long)Hkv);
     DL4S_REQUIRE(d >= 1 && d <= MAXD, DL4S_HIP_EUNSUPPORTED, "%s: head dim %lld (1 to %d are implemented)", what, (long long)d, MAXD);
-    const int64_t big = int64_t(1) << 30;
-    DL4S_REQUIRE(Lq < big && Lk < big && B < big && H < big && B * H < big && desc->q_offset < big, DL4S_HIP_EUNSUPPORTED,
-                 "%s: an extent or the offset above 2^30", what);
+    const int64_t big = int64_t(1) << 30, most = big - 256;
+    DL4S_REQUIRE(Lq <= most && Lk <= most && B < big && H < big && B * H < big && desc->q_offset <= most - Lq, DL4S_HIP_EUNSUPPORTED,
+                 "%s: more than 2^30 heads, or a position above 2^30 - 256", what);
     DL4S_REQUIRE(H * d <= (int64_t(1) << 22), DL4S_HIP_EUNSUPPORTED, "%s: %lld heads of %lld: a token's heads above 2^22 values", what,
                  (long long)H, (long long)d);
     DL4S_REQUIRE(B * H * Lq < big * 4 && B * Hkv * Lk < big * 4, DL4S_HIP_EUNSUPPORTED, "%s: more than 2^32 rows", what);
@@ -411,9 +416,11 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
         return few_rows(ctx, q, k, v, out, stats, B, H, Hkv, Lq, Lk, d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d));
     if (d <= 128) {
         const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
+        if (const int bad = fits_a_launch("sdpa_window_fwd", 8ll * g.per_xcd, 256)) return bad;
         return d % 4 == 0 && on_16_bytes({q, k, v, out}) ? launch_fwd_width<true>(ctx, q, k, v, out, stats, g)
                                                          : launch_fwd_width<false>(ctx, q, k, v, out, stats, g);
     }
+    if (const int bad = fits_a_launch("sdpa_window_fwd", (rows + 3) / 4, 256)) return bad;
     hipLaunchKernelGGL(sdpa_window_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, k, v, out, stats, (int)H, (int)(H / Hkv),
                        (int)Lq, (int)Lk, (int)d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d), rows);
     return dl4s::launch_status("sdpa_window_rows_f32");
@@ -438,6 +445,8 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     if (d <= 128 && H > 0) {
         const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
         KeyBlocks kb = krows ? key_blocks(ctx, g, B) : KeyBlocks{};
+        rc = fits_a_launch("sdpa_window_bwd", std::max(8ll * g.per_xcd, 16ll * (kb.per_xcd[0] + kb.per_xcd[1])), 256);
+        if (rc) return rc;
         rc = dl4s::ensure_scratch(ctx, delta_bytes + reinterpret_cast<size_t>(kb.partial));
         if (rc) return rc;
         float *delta = reinterpret_cast<float *>(ctx->scratch);
@@ -446,7 +455,8 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
                    ? launch_bwd_width<true>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb)
                    : launch_bwd_width<false>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
     }
-    rc = dl4s::ensure_scratch(ctx, delta_bytes);
+    rc = fits_a_launch("sdpa_window_bwd", std::max(rows + 3, krows + 3) / 4, 256);
+    if (!rc) rc = dl4s::ensure_scratch(ctx, delta_bytes);
     if (rc) return rc;
     float *delta = reinterpret_cast<float *>(ctx->scratch);
     if (rows) {

@@ -7,7 +7,7 @@
 //     group.  Two wavefronts share 32 keys (the columns of their accumulators): one holds K and forms S = Q . K^T, the weights
 //     w, and dV^T += dO^T . w, the other holds V and forms dP = dO . V^T and, with the weights it gets through LDS,
 //     dK^T += Q^T . dS.  That halves what a wavefront keeps in registers, so two run on a SIMD at every head dim (one
-//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes 427 us at B2 H16/4 L4096 d96 window 777).
+//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes 436 us at B2 H16/4 L4096 d96 window 777).
 //     Shared key heads are summed in the accumulators, in a fixed order, without atomics.  Key blocks that hold visible
 //     first keys are seen by every later query: their query tiles are dealt to several workgroups whose partial sums a
 //     last kernel adds up in order; so are all blocks where that shortens the longest queue of a compute unit.
@@ -20,42 +20,44 @@
 
 namespace {
 
-// The power of two that an operand carries in a lane's column, and the factor that goes with it.
+// The power of two that an operand carries in a lane's column: the operand is x * factor, factor = base * 2^c.  fit and
+// fit_tiny look at a tile's x before they are multiplied, whose size is that of fp32 numbers, and return whether any lane's power
+// moved; acc_factor is then the lane's factor for what it has accumulated.
 struct ColumnScale {
+    const float base;
+    float factor;
     int c = 0;
     bool fresh = true;
-    // The same for weights, which are at most 2^13: a column takes a power only where its first largest is below 2^-3.
-    __device__ __forceinline__ bool fit_tiny(f32x16 &w, float &factor, float &acc_factor) {
+    __device__ __forceinline__ explicit ColumnScale(const float b) : base(b), factor(b) {}
+
+    // the largest, m, to 2^8
+    __device__ __forceinline__ void move(const bool moves, const float m, const int least, float &acc_factor) {
+        const int to = moves ? min(max(135 - (int)(__float_as_uint(m * base) >> 23), least), 126) : c;
+        acc_factor = pow2(to - c);
+        c = to;
+        factor = base * pow2(c);
+    }
+    __device__ __forceinline__ bool fit(const f32x16 &x, float &acc_factor) {
+        float m = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(x[r]));
+        if (!__any(m * factor > 32768.0f || (fresh && m > 0.f))) return false;
+        m = max_halves(m);
+        const bool moves = m * factor > 32768.0f || (fresh && m > 0.f);
+        fresh = fresh && !(m > 0.f);
+        move(moves, m, -126, acc_factor);
+        return true;
+    }
+    // For weights, which are at most 2^13: a column takes a power only where its first largest is below 2^-3.
+    __device__ __forceinline__ bool fit_tiny(const f32x16 &w, float &acc_factor) {
         float m = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, w[r]);
         m = max_halves(m);
-        const bool move = (c != 0 && m > 32768.0f) || (fresh && m > 0.f && m < 0.125f);
+        const bool moves = (c != 0 && m * factor > 32768.0f) || (fresh && m > 0.f && m < 0.125f);
         fresh = fresh && !(m > 0.f);
-        if (!__any(move)) return false;
-        // the largest to 2^8, with no power below zero
-        const int shift = !move ? 0 : max(min(135 - (int)(__float_as_uint(m) >> 23), 126), -c);
-        c += shift;
-        acc_factor = pow2(shift);
-        factor *= acc_factor;
-        w *= acc_factor;
-        return true;
-    }
-    // ds: this tile's values under the present power.  Returns whether any lane's power moved; acc_factor is then the lane's
-    // factor for what it has accumulated.
-    __device__ __forceinline__ bool fit(f32x16 &ds, float &factor, float &acc_factor) {
-        float m = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(ds[r]));
-        if (!__any(m > 32768.0f || (fresh && m > 0.f))) return false;
-        m = max_halves(m);
-        const bool move = m > 32768.0f || (fresh && m > 0.f);
-        const int shift = move ? min(max(135 - (int)(__float_as_uint(m) >> 23), -126), 126) : 0;
-        fresh = fresh && !(m > 0.f);
-        c += shift;
-        acc_factor = pow2(shift);
-        factor *= acc_factor;
-        ds *= acc_factor;
+        if (!__any(moves)) return false;
+        move(moves, m, 0, acc_factor);
         return true;
     }
 };
@@ -107,9 +109,8 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-    ColumnScale scale;
-    float factor = inv;                                    // dS as an operand = 2^(s - m) (dP - delta) factor
-    int nk = -63;                                          // acc is in units of 2^nk
+    ColumnScale scale(inv);                                // dS = 2^(s - m) (dP - delta) / l
+    int nk = -MOST_POWER;                                          // acc is in units of 2^nk
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
@@ -127,12 +128,11 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
         const Powers kn(powers[0]);
         const i32x4 vn = *reinterpret_cast<const i32x4 *>(powers[1]);
         settle(s, dp);
-        const float del_f = del * factor;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            const float f = __builtin_ldexpf(unq, kn.n[x]), fp = __builtin_ldexpf(ung, vn[x]) * factor;
+            const float f = __builtin_ldexpf(unq, kn.n[x]), fp = __builtin_ldexpf(ung, vn[x]);
 #pragma unroll
-            for (int r = 4 * x; r < 4 * x + 4; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], f, -m)) * __builtin_fmaf(dp[r], fp, -del_f);
+            for (int r = 4 * x; r < 4 * x + 4; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], f, -m)) * __builtin_fmaf(dp[r], fp, -del);
         }
         if (!tile_open(g.w, p0, p1, k0, at.len)) {
 #pragma unroll
@@ -144,13 +144,13 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
             for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
         }
         float shrink;
-        if (scale.fit(s, factor, shrink)) {
+        if (scale.fit(s, shrink)) {
 #pragma unroll
             for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
         }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            const Frag df = acc_frag(s, st);
+            const Frag df = acc_frag(s, st, scale.factor);
             Frag kc[DT / 32];
 #pragma unroll
             for (int t = 0; t < DT / 32; ++t) kc[t] = T::cols_frag(Kc, t, st);
@@ -161,14 +161,15 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t) settle(acc[t]);
     if (at.qi >= g.Lq) return;
-    const float f0 = pow2(-scale.c), f1 = pow2(nk);
+    const int power = nk - scale.c;
     const bool empty = inv == 0.f;                         // saw no key: no gradient, whatever stands in its rows
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             f32x4 x = {acc[t][4 * r], acc[t][4 * r + 1], acc[t][4 * r + 2], acc[t][4 * r + 3]};
-            x = ((x * f0) * f1) * g.rT;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_ldexpf(x[e], power) * g.rT;
             if (empty) x = f32x4{0.f, 0.f, 0.f, 0.f};
             store4(dq + el, 32 * t + 8 * r + 4 * half, g.d, VEC, x);
         }
@@ -274,10 +275,9 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     // The operands are 2^13 w, times a power of two where a column's weights are all tiny, and w (dP - delta) factor.
-    ColumnScale scale;
-    float factor = values ? 1.0f / 8192 : 1.0f;
+    ColumnScale scale(values ? 1.0f / 8192 : 1.0f);
     bool plain = false;                                    // every column has met a weight that needs no power
-    int unit_power = -63;                                  // acc is in units of 2^unit_power
+    int unit_power = -MOST_POWER;                                  // acc is in units of 2^unit_power
 
     // Two buffers: behind the exchange of the weights one wavefront of a pair multiplies and then stages its share of the next
     // tile, the other stages first, so that on their SIMD one's vector work runs beside the other's matrix instructions.
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
                     const f32x4 w = weights[(two * 4 + x) * 64 + lane];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        const float ds = (w[y] * s[4 * x + y]) * factor;
+                        const float ds = w[y] * s[4 * x + y];
                         s[4 * x + y] = w[y] == 0.f ? 0.f : ds;           // (whatever stands in a query's rows that does not see the key)
                     }
                 }
@@ -348,12 +348,12 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
                 for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
             }
             if (values || !plain) {
-                if (!values) s *= factor;
                 float shrink;
-                if (values ? scale.fit(s, factor, shrink) : scale.fit_tiny(s, factor, shrink)) {
+                if (values ? scale.fit(s, shrink) : scale.fit_tiny(s, shrink)) {
 #pragma unroll
                     for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
                 }
+                s *= scale.factor;
                 plain = !__any(scale.fresh || scale.c != 0);
             }
 #pragma unroll
@@ -373,7 +373,8 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
     for (int t = 0; t < DT / 32; ++t) settle(acc[t]);
     if (key >= g.Lk) return;
     // q was staged as q rT log2(e): dk = rT sum dS q = ln(2) of what was summed
-    const float f0 = pow2((values ? 0 : -13) - scale.c) * (values ? 0.69314718055994530942f : 1.0f), f1 = pow2(unit_power);
+    const int power = unit_power - scale.c - (values ? 0 : 13);
+    const float factor_out = values ? 0.69314718055994530942f : 1.0f;
     float *to_row = (values ? dk : dv) + el;
     if (kb.chunks[cl] > 1) to_row = partial_sums(kb, pair, block, chunk, g.d) + (values ? 0 : 128ll * g.d) + (two * 32 + ln) * (long long)g.d;
 #pragma unroll
@@ -381,7 +382,9 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             f32x4 x = {acc[t][4 * r], acc[t][4 * r + 1], acc[t][4 * r + 2], acc[t][4 * r + 3]};
-            store4(to_row, 32 * t + 8 * r + 4 * half, g.d, VEC, (x * f0) * f1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_ldexpf(x[e] * factor_out, power);
+            store4(to_row, 32 * t + 8 * r + 4 * half, g.d, VEC, x);
         }
 }
 

@@ -2,9 +2,10 @@
 //
 // A value x is held as two fp16 planes of x times a power of two, x 2^a = h + l with h = fp16(x 2^a), l = fp16(x 2^a - h),
 // each rounded to nearest: 11 + 11 significant bits.  A product is three matrix instructions, l.h + h.l + h.h (the small ones
-// first), summed in fp32; the one left out is below 2^-22 of the product.  The power of two puts the largest finite value of
-// what shares it (a row for an operand in registers, the tiles seen so far for one in LDS) at 2^14 or more, so a value 2^28
-// times smaller still has all its bits, a smaller one an error of 2^-39 of that largest, and nothing overflows.  Measured
+// first), summed in fp32; the one left out is below 2^-22 of the product.  The power of two is shared: by a row for an operand
+// in registers, whose largest finite value it puts at 2^14 or more, and by what a wavefront has staged so far for one in
+// LDS (2^11 or more).  Nothing overflows, and what a value loses is 2^-23 of it or, where that is more, 2^-39 (2^-36) of
+// that largest: a tensor whose rows differ by up to 2^13 in size is as exact as in fp32 row by row.  Measured
 // against 64 bits, sums of 64 (512) products of normal values are off by 1.2e-7 (2.5e-7) of their size this way, 1.5e-7
 // (3.8e-7) through v_mfma_f32_32x32x2_f32.  Why: a 32 x 32 x 16 step costs 3 x 39 SIMD cycles (measured) where eight fp32
 // steps cost 8 x 66, and the vector ALU runs beside the fp16 instructions, not beside the fp32 ones.  Three bf16 planes
@@ -30,7 +31,7 @@ constexpr int MAXD = 256;
 
 __device__ __forceinline__ float exp2_fast(const float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Positions are below 2^31 (offset and extents below 2^30), so all comparisons are 32-bit.
+// Positions and extents are below 2^30, so that a position and a window add up in 32 bits.
 struct WindowArgs {
     int window, sinks;      // clamped to [1, 2^30] and [0, Lk]
     int q_offset;
@@ -86,17 +87,17 @@ __device__ __forceinline__ void store4(float *row, const int col, const int d, c
 
 // ---- powers of two
 __device__ __forceinline__ float pow2(const int a) { return __builtin_ldexpf(1.0f, a); }
-// The power that puts m (>= 0, finite) into [2^14, 2^15).  m below 2^-49 stays below: two such powers and the scores they
-// belong to keep within the range of fp32, and what is lost are bits below 2^-73.
+// The power that puts m (>= 0, finite) into [2^14, 2^15).  m below 2^-112 stays below, so that the power and its inverse are
+// normal numbers: what is lost there are bits below 2^-136.
 __device__ __forceinline__ int scale_of(const float m) {
     const int e = (int)(__float_as_uint(m) >> 23);
-    return 141 - min(max(e, 78), 254);
+    return 141 - min(max(e, 15), 254);
 }
-// The same in steps of 2^8 ([2^7, 2^15)): neighbouring rows of like size then mostly have the same power.
+// The same in steps of 2^4 ([2^11, 2^15)): neighbouring rows of like size then mostly have the same power.
 __device__ __forceinline__ int coarse_scale_of(const float m) {
-    const int e = (int)(__float_as_uint(m) >> 23);
-    return 141 - min(((max(e, 78) + 3) & ~7) + 4, 256);
+    return 139 - ((max((int)(__float_as_uint(m) >> 23), 15) + 1) & ~3);
 }
+constexpr int MOST_POWER = 123;                            // the largest of these
 __device__ __forceinline__ float finite_abs(const float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
 template <int CTRL>
 __device__ __forceinline__ float max_lanes(const float v) {
@@ -307,7 +308,7 @@ struct Stage {
     f32x4 x[NP][4];
     unsigned from[NP];       // byte offset of the thread's piece in its tensor's tile
     int to_row[NP], to_col[NP];
-    int run[2] = {63, 63};   // smallest power so far of the rows this wavefront stages of either tile
+    int run[2] = {MOST_POWER, MOST_POWER};   // smallest power so far of the rows this wavefront stages of either tile
 
     const int tid, wave0;    // the thread's number, and its wavefront's first, in the order in which wavefronts are given pieces
 
@@ -419,12 +420,20 @@ __device__ __forceinline__ float to_one_unit(const Powers &p, int &n, f32x16 &op
 // Row of register r of a 32 x 32 accumulator in the lane's half of the wavefront (the column is lane % 32).
 __device__ __forceinline__ constexpr int acc_row(const int r) { return 8 * (r >> 2) + (r & 3); }
 
-// The registers [8 step, 8 step + 8) of an accumulator as the other operand of a product that contracts over its rows.
+// The registers [8 step, 8 step + 8) of an accumulator as the other operand of a product that contracts over its rows; in the
+// second form times a factor.
 __device__ __forceinline__ Frag acc_frag(const f32x16 &s, const int step) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = s[8 * step + e];
     return split8(x);
+}
+__device__ __forceinline__ Frag acc_frag(const f32x16 &s, const int step, const float factor) {
+    Planes w[4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        split4(f32x4{s[8 * step + 4 * e], s[8 * step + 4 * e + 1], s[8 * step + 4 * e + 2], s[8 * step + 4 * e + 3]}, factor, w[2 * e], w[2 * e + 1]);
+    return Frag{__builtin_bit_cast(f16x8, (u32x4){w[0].h, w[1].h, w[2].h, w[3].h}), __builtin_bit_cast(f16x8, (u32x4){w[0].l, w[1].l, w[2].l, w[3].l})};
 }
 
 }  // namespace

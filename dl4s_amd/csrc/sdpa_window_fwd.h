@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
     float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
-    int nv = -63;                                          // o is in units of 2^nv
+    int nv = -MOST_POWER;                                          // o is in units of 2^nv
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
@@ -120,11 +120,11 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = sees(g.w, p, k0 + acc_row(r) + 4 * half, at.len) ? s[r] : -INFINITY;
             }
-            // scores = accumulators * f, one factor for every eight keys
+            // scores = accumulators * f, one factor for every eight keys (not zero, for those at -inf)
             float f[4], tmax = -INFINITY;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                f[x] = __builtin_ldexpf(unq, nk[x]);
+                f[x] = fmaxf(__builtin_ldexpf(unq, nk[x]), 1.17549435e-38f);
                 tmax = fmaxf(tmax, fmaxf(fmaxf(s[4 * x], s[4 * x + 1]), fmaxf(s[4 * x + 2], s[4 * x + 3])) * f[x]);
             }
             // the reference maximum moves, and the sums are rescaled, only when a weight would pass 2^8 (x 2^7): any factor
