@@ -149,6 +149,7 @@ int launch_rotary(dl4s_hip_ctx *ctx, const float *q, float *q_out, const float *
     if (a.rot) a.per_wg = std::max(1, std::min(a.per_wg, 32768 / (a.rot * 4)));
     const size_t lds = (size_t)a.per_wg * (a.rot / 2) * sizeof(f32x2);
     const dim3 grid((a.tokens + a.per_wg - 1) / a.per_wg);
+    DL4S_REQUIRE(grid.x < (1u << 24), DL4S_HIP_EUNSUPPORTED, "rotary: %u workgroups of 256 threads", grid.x);
     if (vec) hipLaunchKernelGGL((rotary_f32<APPEND, true>), grid, dim3(256), lds, ctx->stream, q, q_out, k, k_out, v, v_out, a);
     else hipLaunchKernelGGL((rotary_f32<APPEND, false>), grid, dim3(256), lds, ctx->stream, q, q_out, k, k_out, v, v_out, a);
     return dl4s::launch_status("rotary_f32");
@@ -165,7 +166,7 @@ int rotary_checks(const char *what, int64_t B, int64_t L, int64_t H, int64_t Hkv
     const int64_t big = int64_t(1) << 30;
     DL4S_REQUIRE(B < big && L < big && H < big && Hkv < big && position0 > -big && position0 < big, DL4S_HIP_EUNSUPPORTED,
                  "%s: an extent or the first position above 2^30", what);
-    DL4S_REQUIRE(B * L < big && (H + Hkv) * d < big, DL4S_HIP_EUNSUPPORTED, "%s: more than 2^30 tokens or columns of a token", what);
+    DL4S_REQUIRE(B * L < big && (H + Hkv) * d < big / 2, DL4S_HIP_EUNSUPPORTED, "%s: more than 2^30 tokens or 2^29 columns of a token", what);
     return DL4S_HIP_OK;
 }
 
