@@ -345,12 +345,13 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_f32(const float *x, co
     }
 }
 
-int logprob_checks(const char *what, int64_t rows, int64_t n, int64_t stride, const float *logits) {
+int logprob_checks(const char *what, int64_t rows, int64_t n, int64_t stride, const float *logits, float t) {
     DL4S_REQUIRE(rows >= 0 && n >= 0, DL4S_HIP_EINVALID_ARG, "%s: negative extent", what);
     if (rows == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE(logits, DL4S_HIP_EINVALID_ARG, "%s: NULL logits", what);
     DL4S_REQUIRE(n >= 1 && n < (int64_t(1) << 31) && rows < (int64_t(1) << 31), DL4S_HIP_EUNSUPPORTED,
                  "%s: %lld rows of %lld tokens (rows of 1 to 2^31 - 1 tokens are implemented)", what, (long long)rows, (long long)n);
+    DL4S_REQUIRE(t > 0.f || t < 0.f, DL4S_HIP_EINVALID_ARG, "%s: inv_temperature %g (it may not be zero)", what, (double)t);
     DL4S_REQUIRE(stride >= n, DL4S_HIP_ESHAPE, "%s: rows of %lld tokens every %lld floats", what, (long long)n, (long long)stride);
     return DL4S_HIP_OK;
 }
@@ -374,7 +375,7 @@ int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t 
                                 float inv_temperature, const int32_t *targets, int32_t ignore_index, float *logprobs, float *entropy,
                                 float *stats, int64_t top_k, float *top_logprobs, int32_t *top_tokens) {
     DL4S_CHECK_CTX(ctx);
-    int rc = logprob_checks("token_logprobs", rows, n, row_stride, logits);
+    int rc = logprob_checks("token_logprobs", rows, n, row_stride, logits, inv_temperature);
     if (rc || rows == 0) return rc;
     DL4S_REQUIRE((targets != nullptr) == (logprobs != nullptr), DL4S_HIP_EINVALID_ARG,
                  "token_logprobs: targets and logprobs come together");
@@ -428,7 +429,7 @@ int dl4s_hip_token_logprobs_bwd_f32(dl4s_hip_ctx *ctx, const float *logits, int6
                                     float inv_temperature, const int32_t *targets, int32_t ignore_index, const float *stats,
                                     const float *dlogprobs, const float *dentropy, float *dlogits) {
     DL4S_CHECK_CTX(ctx);
-    const int rc = logprob_checks("token_logprobs_bwd", rows, n, row_stride, logits);
+    const int rc = logprob_checks("token_logprobs_bwd", rows, n, row_stride, logits, inv_temperature);
     if (rc || rows == 0) return rc;
     DL4S_REQUIRE(stats && dlogits, DL4S_HIP_EINVALID_ARG, "token_logprobs_bwd: NULL pointer");
     DL4S_REQUIRE(!dlogprobs || targets, DL4S_HIP_EINVALID_ARG, "token_logprobs_bwd: a gradient of the log probabilities without targets");
