@@ -14,68 +14,6 @@
 
 namespace {
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
-}
-
-// One wavefront per query row, 64 keys at a time: a lane forms the score of one key, then a lane owns up to four output
-// columns.  Any head dim up to 256, any alignment.
-__global__ __launch_bounds__(256) void sdpa_window_rows_f32(const float *__restrict__ q, const float *__restrict__ k,
-                                                             const float *__restrict__ v, float *__restrict__ out,
-                                                             float *__restrict__ stats, int H, int group, int Lq, int Lk, int d,
-                                                             float rT, WindowArgs w, Layout lq, Layout lk, long long rows) {
-    __shared__ float qs[4][MAXD], ps[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long row = (long long)blockIdx.x * 4 + wave;
-    if (row >= rows) return;
-    const int i = (int)(row % Lq);
-    const long long bh = row / Lq;
-    const int h = (int)(bh % H), b = (int)(bh / H);
-    const float *qp = q + b * lq.b + h * lq.h + i * lq.l;
-    const float *kp = k + b * lk.b + (h / group) * lk.h, *vp = v + b * lk.b + (h / group) * lk.h;
-    for (int c = lane; c < d; c += 64) qs[wave][c] = qp[c] * rT;
-    const Range r = visible_keys(w, b, i, Lk);
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int part = 0; part < 2; ++part) {
-        const int end = part ? r.hi : r.first;
-        for (int j0 = part ? r.lo : 0; j0 < end; j0 += 64) {
-            const int n = min(64, end - j0);
-            float s = -INFINITY;
-            if (lane < n) {
-                const float *kr = kp + (long long)(j0 + lane) * lk.l;
-                s = 0.f;
-                for (int c = 0; c < d; ++c) s += qs[wave][c] * kr[c];
-                s *= LOG2E;
-            }
-            const float m_new = fmaxf(m, wave_max(s));
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = __builtin_amdgcn_exp2f(m - m_use), p = lane < n ? __builtin_amdgcn_exp2f(s - m_use) : 0.f;
-            m = m_new;
-            l = l * alpha + dl4s::wave_sum(p);
-            ps[wave][lane] = p;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int c = lane + 64 * t;
-                if (c >= d) break;
-                float a = acc[t] * alpha;
-                for (int x = 0; x < n; ++x) a += ps[wave][x] * vp[(long long)(j0 + x) * lk.l + c];
-                acc[t] = a;
-            }
-        }
-    }
-    const float inv = r.first + (r.hi - r.lo) > 0 ? 1.0f / l : 0.f;
-    float *op = out + b * lq.b + h * lq.h + i * lq.l;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-        if (lane + 64 * t < d) op[lane + 64 * t] = acc[t] * inv;
-    if (stats && lane == 0) {
-        stats[2 * row] = m == -INFINITY ? 0.f : m;
-        stats[2 * row + 1] = inv;
-    }
-}
-
 // delta_i = dout_i . out_i, one wavefront per row
 __global__ __launch_bounds__(256) void window_delta_f32(const float *__restrict__ dout, const float *__restrict__ out,
                                                          float *__restrict__ delta, int H, int Lq, int d, Layout lq, long long rows) {
@@ -326,48 +264,56 @@ int launch_bwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const fl
 }
 
 // Few query rows: the workgroups and the split of the keys.  Lk is the number of rows that can be visible at all (T of a cache).
-template <int DT, int NW>
-int launch_few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, FewArgs &a, int64_t pairs) {
-    const int most_cols = std::min(16, a.cols);
-    const size_t of_row = (size_t)NW * (DT + 4) * sizeof(float), lds = most_cols * of_row;
-    const int rc = lds_limit(ctx, dl4s::LDS_WINDOW_FEW, DT == 64 ? 0 : (DT == 128 ? 1 : 2), sdpa_window_few_f32<DT, NW>, 16 * of_row);
-    if (rc) return rc;
-    hipLaunchKernelGGL((sdpa_window_few_f32<DT, NW>), dim3(a.nsplit, (unsigned)pairs, (a.cols + 15) / 16), dim3(NW * 64), lds, ctx->stream, q, k,
-                       v, out, stats, a);
-    return dl4s::launch_status("sdpa_window_few_f32");
-}
-
-int few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, int64_t B, int64_t H, int64_t Hkv,
-             int64_t Lq, int64_t Lk, int64_t d, float rT, const WindowArgs &w, Layout lq, Layout lk) {
+FewArgs few_args(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float rT, const WindowArgs &w, Layout lq, Layout lk,
+                 int cus) {
     FewArgs a;
     a.H = (int)H; a.Hkv = (int)Hkv; a.group = (int)(H / Hkv); a.Lq = (int)Lq; a.Lk = (int)Lk; a.d = (int)d;
     a.cols = a.group * a.Lq;
     a.rT = rT;
-    a.vec = d % 4 == 0 && on_16_bytes({q, k, v});
     a.lq = lq; a.lk = lk; a.w = w;
-    const int64_t pairs = B * Hkv;
-    // Workgroups of 8 wavefronts.  Enough of them that every compute unit has one; a split costs a second launch, so up to
-    // 512 keys one workgroup reads them all, and a workgroup has at least 256 keys.
-    const int NW = 8;
-    const int64_t most = std::min<int64_t>(Lk, (int64_t)w.window + Lq - 1 + w.sinks), blocks = pairs * ((a.cols + 15) / 16);
-    int64_t ns = most <= 512 ? 1 : std::min<int64_t>(MAX_SPLIT, std::min((ctx->cu_count + blocks - 1) / blocks, (most + 255) / 256));
+    // Workgroups of 8 wavefronts and 16 rows.  Enough of them that every compute unit has one; a split costs a second launch, so
+    // up to 512 keys one workgroup reads them all, and a workgroup has at least 256 keys.
+    const int64_t queries = std::min<int64_t>(Lq, 14 / a.group + 2);         // of a workgroup's rows
+    const int64_t most = std::min<int64_t>(Lk, (int64_t)w.window + queries - 1 + w.sinks), blocks = B * Hkv * ((a.cols + 15) / 16);
+    const int64_t ns = most <= 512 ? 1 : std::min<int64_t>(MAX_SPLIT, std::min((cus + blocks - 1) / blocks, (most + 255) / 256));
     a.chunk = (int)std::max<int64_t>(16, ((most + ns - 1) / ns + 15) / 16 * 16);
     a.nsplit = (int)std::max<int64_t>(1, (most + a.chunk - 1) / a.chunk);
     a.partial = nullptr;
+    a.pair0 = 0;
+    return a;
+}
+
+template <int DT>
+int launch_few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, FewArgs &a, int64_t pairs) {
+    constexpr int NW = 8;
+    const size_t of_row = (size_t)NW * (DT + 4) * sizeof(float), lds = std::min(16, a.cols) * of_row;
+    const long long workgroups = (long long)a.nsplit * ((a.cols + 15) / 16);
+    int rc = fits_a_launch("sdpa_window", workgroups, NW * 64);
+    if (!rc) rc = lds_limit(ctx, dl4s::LDS_WINDOW_FEW, DT == 64 ? 0 : (DT == 128 ? 1 : 2), sdpa_window_few_f32<DT, NW>, 16 * of_row);
+    for (int64_t from = 0; from < pairs && !rc; from += 65535) {
+        const unsigned n = (unsigned)std::min<int64_t>(pairs - from, 65535);
+        a.pair0 = (int)from;
+        hipLaunchKernelGGL((sdpa_window_few_f32<DT, NW>), dim3((unsigned)workgroups, n), dim3(NW * 64), lds, ctx->stream, q, k, v, out, stats, a);
+        rc = dl4s::launch_status("sdpa_window_few_f32");
+        if (rc || a.nsplit == 1) continue;
+        hipLaunchKernelGGL(sdpa_window_merge_f32, dim3(a.cols, n), dim3(MAX_SPLIT), 0, ctx->stream, out, stats, a);
+        rc = dl4s::launch_status("sdpa_window_merge_f32");
+    }
+    return rc;
+}
+
+int few_rows(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, FewArgs &a, int64_t pairs) {
+    a.vec = a.d % 4 == 0 && on_16_bytes({q, k, v});
     std::unique_lock<std::mutex> scratch_lock(ctx->scratch_mu, std::defer_lock);
-    int rc;
     if (a.nsplit > 1) {
         scratch_lock.lock();
-        rc = dl4s::ensure_scratch(ctx, (size_t)pairs * a.nsplit * a.cols * (d + 2) * sizeof(float));
+        const int rc = dl4s::ensure_scratch(ctx, (size_t)pairs * a.nsplit * a.cols * (a.d + 2) * sizeof(float));
         if (rc) return rc;
         a.partial = reinterpret_cast<float *>(ctx->scratch);
     }
-    if (d <= 64) rc = launch_few_rows<64, NW>(ctx, q, k, v, out, stats, a, pairs);
-    else if (d <= 128) rc = launch_few_rows<128, NW>(ctx, q, k, v, out, stats, a, pairs);
-    else rc = launch_few_rows<256, NW>(ctx, q, k, v, out, stats, a, pairs);
-    if (rc || a.nsplit == 1) return rc;
-    hipLaunchKernelGGL(sdpa_window_merge_f32, dim3(a.cols, (unsigned)pairs), dim3(MAX_SPLIT), 0, ctx->stream, out, stats, a);
-    return dl4s::launch_status("sdpa_window_merge_f32");
+    if (a.d <= 64) return launch_few_rows<64>(ctx, q, k, v, out, stats, a, pairs);
+    if (a.d <= 128) return launch_few_rows<128>(ctx, q, k, v, out, stats, a, pairs);
+    return launch_few_rows<256>(ctx, q, k, v, out, stats, a, pairs);
 }
 
 // What the three entry points check alike.  Returns a status; *w is filled in.
@@ -411,19 +357,19 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     if (rows == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE(q && out && (Lk == 0 || (k && v)), DL4S_HIP_EINVALID_ARG, "sdpa_window_fwd: NULL tensor pointer");
     const bool tm = flags & DL4S_SDPA_TOKEN_MAJOR;
-    // few rows to a key head: the matrix kernels' tiles of 32 rows would be mostly empty, and their keys are not split
-    if (H / Hkv * Lq <= 32 && B * Hkv <= 65535)
-        return few_rows(ctx, q, k, v, out, stats, B, H, Hkv, Lq, Lk, d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d));
-    if (d <= 128) {
-        const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
-        if (const int bad = fits_a_launch("sdpa_window_fwd", 8ll * g.per_xcd, 256)) return bad;
-        return d % 4 == 0 && on_16_bytes({q, k, v, out}) ? launch_fwd_width<true>(ctx, q, k, v, out, stats, g)
-                                                         : launch_fwd_width<false>(ctx, q, k, v, out, stats, g);
-    }
-    if (const int bad = fits_a_launch("sdpa_window_fwd", (rows + 3) / 4, 256)) return bad;
-    hipLaunchKernelGGL(sdpa_window_rows_f32, row_grid(rows), dim3(256), 0, ctx->stream, q, k, v, out, stats, (int)H, (int)(H / Hkv),
-                       (int)Lq, (int)Lk, (int)d, inv_temperature, w, layout(tm, H, Lq, d), layout(tm, Hkv, Lk, d), rows);
-    return dl4s::launch_status("sdpa_window_rows_f32");
+    const Layout lq = layout(tm, H, Lq, d), lk = layout(tm, Hkv, Lk, d);
+    // The kernel for few rows takes 16 to a workgroup and shares their keys among wavefronts and workgroups; the other takes 128
+    // and walks their keys in turn, on faster instructions.  While a compute unit gets at most one workgroup of the former it
+    // is the faster one (d 64: 8 heads L 512 window 256 11 us against 22, 64 rows over 4096 keys 17 against 165, 512 workgroups
+    // of a group of four 19 against 19, 1024 of them 36 against 19), as for 16 rows to a key head over long stretches (1024
+    // key heads, 2048 keys: 180 us against 219, 500 keys: 64 against 60).  Above 128 columns it is the only one.
+    FewArgs few = few_args(B, H, Hkv, Lq, Lk, d, inv_temperature, w, lq, lk, ctx->cu_count);
+    const int64_t blocks = B * Hkv * ((few.cols + 15) / 16), most = std::min<int64_t>(Lk, (int64_t)w.window + w.sinks);
+    if (d > 128 || blocks <= ctx->cu_count || (few.cols <= 16 && most > 1024)) return few_rows(ctx, q, k, v, out, stats, few, B * Hkv);
+    const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
+    if (const int bad = fits_a_launch("sdpa_window_fwd", 8ll * g.per_xcd, 256)) return bad;
+    return d % 4 == 0 && on_16_bytes({q, k, v, out}) ? launch_fwd_width<true>(ctx, q, k, v, out, stats, g)
+                                                     : launch_fwd_width<false>(ctx, q, k, v, out, stats, g);
 }
 
 int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
@@ -483,11 +429,9 @@ int dl4s_hip_sdpa_window_decode_f32(dl4s_hip_ctx *ctx, const float *q, const flo
     if (B * H == 0) return DL4S_HIP_OK;
     DL4S_REQUIRE(q && kcache && vcache && out, DL4S_HIP_EINVALID_ARG, "sdpa_window_decode: NULL tensor pointer");
     DL4S_REQUIRE(T >= 1 && T <= Tcap, DL4S_HIP_ESHAPE, "sdpa_window_decode: T=%lld must be in [1, Tcap=%lld]", (long long)T, (long long)Tcap);
-    DL4S_REQUIRE(B * Hkv <= 65535 && H / Hkv <= (1 << 20), DL4S_HIP_EUNSUPPORTED,
-                 "sdpa_window_decode: B*Hkv=%lld above 65535, or more than 2^20 query heads to a key head", (long long)(B * Hkv));
     w.last_key = 1;
-    return few_rows(ctx, q, kcache, vcache, out, nullptr, B, H, Hkv, 1, T, d, inv_temperature, w, layout(false, H, 1, d),
-                    layout(false, Hkv, Tcap, d));
+    FewArgs a = few_args(B, H, Hkv, 1, T, d, inv_temperature, w, layout(false, H, 1, d), layout(false, Hkv, Tcap, d), ctx->cu_count);
+    return few_rows(ctx, q, kcache, vcache, out, nullptr, a, B * Hkv);
 }
 
 }  // extern "C"

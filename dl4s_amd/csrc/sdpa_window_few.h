@@ -1,4 +1,5 @@
-// Windowed attention for few query rows over many keys: a decoding step over a cache, or the last rows of a prompt.
+// Windowed attention for few query rows: a decoding step over a cache, the last rows of a prompt, short prompts; and the forward
+// pass above 128 columns.
 //
 // What bounds it is reading the visible keys and values once from HBM.  One wavefront takes 16 keys at a time for up to 16
 // query rows of one key head (the heads of a group, and their rows): S[key, row] = K . Q^T and O[column, row] += V^T . P on
@@ -17,12 +18,13 @@
 namespace {
 
 struct FewArgs {
-    int H, Hkv, group, Lq, Lk, d, cols;      // cols = group * Lq query rows of a key head: row c = head c / Lq, query c % Lq
+    int H, Hkv, group, Lq, Lk, d, cols;      // cols = group * Lq query rows of a key head: row c = query c / group, head c % group
     float rT;
     int vec;
     Layout lq, lk;
     WindowArgs w;
     int nsplit, chunk;                       // visible keys per workgroup (a multiple of 16)
+    int pair0;                               // (batch, key head) pair of blockIdx.y = 0
     float *partial;                          // [pair][split][cols][d + 2], with nsplit > 1
 };
 
@@ -31,17 +33,17 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 3 : (DT <= 128 ? 2 : 1)) void s
     const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v, float *__restrict__ out,
     float *__restrict__ stats, const FewArgs a) {
     extern __shared__ __align__(16) float few_lds[];
-    const int split = blockIdx.x, pair = blockIdx.y, c0 = blockIdx.z * 16, nc = min(16, a.cols - c0);
+    const int split = blockIdx.x % a.nsplit, c0 = blockIdx.x / a.nsplit * 16, nc = min(16, a.cols - c0), pair = a.pair0 + blockIdx.y;
     const int hk = pair % a.Hkv, b = pair / a.Hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, ln = lane & 15, quad = lane >> 4;
     const int len = valid_keys(a.w, b, a.Lk);
 
-    // the keys any row of the pair sees: [0, first) and [lo, hi); x counts through both
-    const Range r0 = visible_keys(a.w, b, 0, a.Lk), r1 = visible_keys(a.w, b, a.Lq - 1, a.Lk);
+    // the keys any of these rows sees: [0, first) and [lo, hi); x counts through both
+    const Range r0 = visible_keys(a.w, b, c0 / a.group, a.Lk), r1 = visible_keys(a.w, b, (c0 + nc - 1) / a.group, a.Lk);
     const int lo = r0.lo, first = min(a.w.sinks, lo), hi = r1.hi, seen = first + max(0, hi - lo);
     const int x0 = split * a.chunk, x1 = min(seen, x0 + a.chunk);
 
-    const int col = c0 + min(ln, nc - 1), hq = hk * a.group + col / a.Lq, iq = col % a.Lq;
+    const int col = c0 + min(ln, nc - 1), hq = hk * a.group + col % a.group, iq = col / a.group;
     const int p = a.w.last_key ? len - 1 : a.w.q_offset + iq;
     float qf[DT / 4];
     {
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 3 : (DT <= 128 ? 2 : 1)) void s
             rec[x] = O;
             if (x == 0) { rec[a.d] = M; rec[a.d + 1] = L; }
         } else {
-            const int h = hk * a.group + row / a.Lq, i = row % a.Lq;
+            const int h = hk * a.group + row % a.group, i = row / a.group;
             const Range r = visible_keys(a.w, b, i, a.Lk);
             const float inv = r.first + (r.hi - r.lo) > 0 ? 1.0f / L : 0.f;
             out[b * a.lq.b + h * a.lq.h + i * a.lq.l + x] = O * inv;
@@ -194,8 +196,8 @@ constexpr int MAX_SPLIT = 256;
 // all parts, whose loads do not wait for each other.
 __global__ __launch_bounds__(MAX_SPLIT) void sdpa_window_merge_f32(float *__restrict__ out, float *__restrict__ stats, const FewArgs a) {
     __shared__ float factor[MAX_SPLIT], most[4], total[4];
-    const int row = blockIdx.x, pair = blockIdx.y, x = threadIdx.x, wave = x >> 6;
-    const int hk = pair % a.Hkv, b = pair / a.Hkv, h = hk * a.group + row / a.Lq, i = row % a.Lq;
+    const int row = blockIdx.x, pair = a.pair0 + blockIdx.y, x = threadIdx.x, wave = x >> 6;
+    const int hk = pair % a.Hkv, b = pair / a.Hkv, h = hk * a.group + row % a.group, i = row / a.group;
     const long long step = (long long)a.cols * (a.d + 2);
     const float *rec = a.partial + ((long long)pair * a.nsplit * a.cols + row) * (a.d + 2);
     const float m = x < a.nsplit ? rec[x * step + a.d] : -INFINITY, l = x < a.nsplit ? rec[x * step + a.d + 1] : 0.f;

@@ -225,7 +225,7 @@ def test_training_past_32_bit_offsets(ctx):
 
 @pytest.mark.parametrize("change", [
     dict(H=1 << 15, Hkv=1 << 15, d=256), dict(q_offset=(1 << 30) - 256), dict(Lq=1 << 30), dict(Lk=(1 << 30) - 100),
-    dict(B=1 << 24, Lq=1, Lk=1), dict(B=1 << 18, Lq=400, d=200), dict(B=1 << 29, H=4, Hkv=4)])
+    dict(B=1 << 24, Lq=20, Lk=1), dict(B=1 << 29, H=4, Hkv=4)])
 def test_limits_are_refused(ctx, change):
     """Extents that the kernels' 32-bit positions and offsets, or one launch, do not hold."""
     from dl4s_amd import lib
@@ -240,11 +240,33 @@ def test_limits_are_refused(ctx, change):
     x.release()
 
 
-def test_decoding_limits_are_refused(ctx):
+@pytest.mark.parametrize("B,H,Hkv,d", [(70000, 1, 1, 5), (1, 40000, 1, 8), (66000, 1, 1, 140)])
+def test_very_many_heads(ctx, B, H, Hkv, d):
+    """More (batch, key head) pairs than a grid's second axis has, a group of thousands: decoding and one row of a prompt."""
+    rng = np.random.default_rng(16)
+    q, k, v, _ = _inputs(rng, B, H, Hkv, 1, 3, d)
+    bufs, out = [ctx.to_device(x) for x in (q, k, v)], ctx.empty(q.shape)
+    group = q.reshape(B, Hkv, H // Hkv, d).astype(np.float64)
+    s = (group @ k[:, :, 1:].astype(np.float64).transpose(0, 1, 3, 2)) * 0.2
+    w = np.exp(s - s.max(-1, keepdims=True))
+    w /= w.sum(-1, keepdims=True)
+    want = (w @ v[:, :, 1:]).reshape(q.shape)
+    # worst case of two keys: the scores' errors, their weights', the sum's (window_reference)
+    size = (np.abs(group) @ np.abs(k[:, :, 1:]).transpose(0, 1, 3, 2)).max(-1, keepdims=True) * 0.2
+    bound = 2.0 ** -24 * ((2 * (d + 24) * (1 + size) + 40) * np.abs(v).max((2, 3))[:, :, None, None]).reshape(B, H, 1, 1)
+    for call in (lambda: ctx.sdpa_window_decode(*bufs, out, B, H, Hkv, 3, 3, d, 0.2, 2),
+                 lambda: ctx.sdpa_window_fwd(*bufs, out, None, B, H, Hkv, 1, 3, d, 0.2, ctx.window_desc(2, 0, 2))):
+        ctx.fill(float("nan"), out, B * H * d)
+        call()
+        assert (np.abs(out.numpy() - want) <= bound).all()
+    for x in bufs + [out]:
+        x.release()
+
+
+def test_limits_of_one_launch(ctx):
     from dl4s_amd import lib
     x = ctx.empty((64,))
-    for B, H, Hkv in ((70000, 1, 1), (1, (1 << 20) + 1, 1)):
-        with pytest.raises(lib.Dl4sHipError) as e:
-            ctx.sdpa_window_decode(x, x, x, x, B, H, Hkv, 1, 1, 1, 1.0, 4)
-        assert e.value.code == -5
+    with pytest.raises(lib.Dl4sHipError) as e:            # 2^23 workgroups of 16 rows
+        ctx.sdpa_window_fwd(x, x, x, x, None, 1, 1, 1, 1 << 27, 4, 140, 1.0, ctx.window_desc(4))
+    assert e.value.code == -5
     x.release()
