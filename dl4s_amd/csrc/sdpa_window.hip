@@ -363,9 +363,12 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     // is the faster one (d 64: 8 heads L 512 window 256 11 us against 22, 64 rows over 4096 keys 17 against 165, 512 workgroups
     // of a group of four 19 against 19, 1024 of them 36 against 19), as for 16 rows to a key head over long stretches (1024
     // key heads, 2048 keys: 180 us against 219, 500 keys: 64 against 60).  Above 128 columns it is the only one.
-    FewArgs few = few_args(B, H, Hkv, Lq, Lk, d, inv_temperature, w, lq, lk, ctx->cu_count);
-    const int64_t blocks = B * Hkv * ((few.cols + 15) / 16), most = std::min<int64_t>(Lk, (int64_t)w.window + w.sinks);
-    if (d > 128 || blocks <= ctx->cu_count || (few.cols <= 16 && most > 1024)) return few_rows(ctx, q, k, v, out, stats, few, B * Hkv);
+    const int64_t cols = H / Hkv * Lq, blocks = (cols + 15) / 16, most = std::min<int64_t>(Lk, (int64_t)w.window + w.sinks);
+    if (d > 128 || B * Hkv * blocks <= ctx->cu_count || (cols <= 16 && most > 1024)) {
+        if (const int bad = fits_a_launch("sdpa_window_fwd", blocks, 512)) return bad;
+        FewArgs few = few_args(B, H, Hkv, Lq, Lk, d, inv_temperature, w, lq, lk, ctx->cu_count);
+        return few_rows(ctx, q, k, v, out, stats, few, B * Hkv);
+    }
     const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
     if (const int bad = fits_a_launch("sdpa_window_fwd", 8ll * g.per_xcd, 256)) return bad;
     return d % 4 == 0 && on_16_bytes({q, k, v, out}) ? launch_fwd_width<true>(ctx, q, k, v, out, stats, g)

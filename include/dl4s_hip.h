@@ -297,9 +297,18 @@ int dl4s_hip_argmax_to_f32(dl4s_hip_ctx *ctx, const float *values, int64_t count
  * A row that sees no key (a length of zero, a window that lies behind the last valid key) has output zero and takes part in
  * no gradient.  q, out [B,H,Lq,d], k, v [B,Hkv,Lk,d], or [B,L,heads,d] with DL4S_SDPA_TOKEN_MAJOR; row-major fp32 without
  * gaps.  Hkv divides H, and H / Hkv consecutive query heads read the same key head.  d from 1 to 256, any alignment of the
- * pointers.  The outputs may not overlap the inputs.  K and V are taken to be finite at keys that are hidden from some
- * queries and visible to others of the same 32 (a NaN or infinity there reaches those other rows' neighbours too); rows at
- * or beyond lengths[b] are never used and may hold anything.  An infinite q, k, v or dout gives NaN. */
+ * pointers.  k and v may be one tensor; the outputs may not overlap the inputs.
+ * What stands in masked places: rows at or beyond lengths[b], keys behind the last query's position and keys that lie before
+ * the first query's window (and are none of the first) may hold anything, as may q and dout in rows that see no key.  A key
+ * that some queries see and others do not has to be finite: its weight in the other rows is zero, and zero times NaN or
+ * infinity is NaN there too.  An infinity among the operands of a visible pair gives NaN.
+ * Precision: fp32 throughout; up to 128 columns the products are formed from two fp16 halves of each operand that share a
+ * power of two along a row, or among the rows of k, v, q, dout that are read together, so a value also carries an error of up
+ * to 2^-36 of the largest of those rows (sums of 64 products of like-sized values are off by 1.2e-7 of their size, 1.5e-7
+ * on the fp32 instructions).
+ * Limits (DL4S_HIP_EUNSUPPORTED): H * d up to 2^22, q_offset + Lq and Lk up to 2^30 - 256, B * H below 2^30, fewer than 2^32 rows,
+ * and 2^24 workgroups of a launch (of 128 rows, above 128 columns of 4; half as many of 16 for few rows).  The first call of a
+ * shape may need the library's scratch block to grow, which a recording refuses: run the same call once before. */
 typedef struct dl4s_window_desc {
     int64_t window;         /* >= 1: the query's own position and the window - 1 before it */
     int64_t sinks;          /* >= 0: the first keys, which stay visible to every later position */
@@ -313,7 +322,7 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
                                  const dl4s_window_desc *window, uint32_t flags);
 /* dq, dk, dv for the upstream gradient dout, from the tensors of the forward call with the same extents, window and flags.
  * dk and dv are summed over the query heads that share a key head.  Deterministic: no atomics, the same bits on every run.
- * Uses the library's scratch block. */
+ * Uses the library's scratch block.  Above 128 columns simple kernels without matrix instructions form it. */
 int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
                                  const float *stats, const float *dout, float *dq, float *dk, float *dv, int64_t B, int64_t H,
                                  int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float inv_temperature, const dl4s_window_desc *window,
@@ -321,7 +330,8 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
 /* One decoding step: q, out [B,H,1,d] over caches [B,Hkv,Tcap,d] whose first lengths[b] rows are valid (device int32 [B];
  * NULL: T rows everywhere; values are clamped to [0, T]).  The query stands at the last valid row: it sees the last `window`
  * rows and the first `sinks`.  A length of zero gives zeros.  T is the largest length there can be, so that the call can be
- * recorded once and replayed while the lengths grow in device memory. */
+ * recorded once and replayed while the lengths grow in device memory.  Rows of the caches that are neither in the window nor
+ * among the first may hold anything (an evicted row, one that was never written). */
 int dl4s_hip_sdpa_window_decode_f32(dl4s_hip_ctx *ctx, const float *q, const float *kcache, const float *vcache, float *out, int64_t B,
                                     int64_t H, int64_t Hkv, int64_t T, int64_t Tcap, int64_t d, float inv_temperature, int64_t window,
                                     int64_t sinks, const int32_t *lengths);
@@ -349,15 +359,18 @@ typedef enum dl4s_rotary_scaling {
 } dl4s_rotary_scaling;
 int dl4s_hip_rotary_frequencies(int64_t rot_dim, double base, int scaling, double factor, double low, double high,
                                 int64_t original_length, double *out_turns);
-/* Queries and keys in one launch (either pair of pointers may be NULL with its head count 0); an output may be its input.
- * positions: device int32 [B,L], or NULL for position0 + l. */
+/* Queries and keys in one launch (either pair of pointers may be NULL with its head count 0); an output may be its input, and
+ * may not overlap it otherwise.  positions: device int32 [B,L], or NULL for position0 + l; negative ones turn backwards.  d up to
+ * 4096, B * L below 2^30, (H + Hkv) * d below 2^29. */
 int dl4s_hip_rotary_f32(dl4s_hip_ctx *ctx, const float *q, float *q_out, const float *k, float *k_out, int64_t B, int64_t L, int64_t H,
                         int64_t Hkv, int64_t d, int64_t rot_dim, const double *turns, const int32_t *positions, int64_t position0,
                         float amplitude, uint32_t flags);
 /* L new rows per batch element: turned queries to q_out, turned keys and the values into the caches [B,Hkv,Tcap,d].  The rows
  * of batch element b stand at positions[b] + l (device int32 [B], or NULL for position0 + l), which is also their cache row;
  * only the first counts[b] of them are written when counts (device int32 [B]) is given, and a row outside [0, Tcap) is not
- * written.  The queries of all L rows are turned.  DL4S_ROTARY_INVERSE is refused. */
+ * written.  The queries of all L rows are turned.  Rows of the new tensors and the caches that are not written or not counted are
+ * not looked at.  A batch element's rows stand at different positions by construction, so no cache row is written twice.
+ * DL4S_ROTARY_INVERSE is refused. */
 int dl4s_hip_rotary_append_f32(dl4s_hip_ctx *ctx, const float *q, const float *k_new, const float *v_new, float *q_out, float *kcache,
                                float *vcache, int64_t B, int64_t L, int64_t H, int64_t Hkv, int64_t Tcap, int64_t d, int64_t rot_dim,
                                const double *turns, const int32_t *positions, int64_t position0, const int32_t *counts, float amplitude,
@@ -487,7 +500,8 @@ int dl4s_hip_log_softmax_f32(dl4s_hip_ctx *ctx, const float *x, int64_t rows, in
  *   entropy[r]  = -sum p log p                       a blocked token (z = -inf) adds nothing
  *   top_logprobs, top_tokens [rows, top_k]           the top_k largest z of the row in order, equal ones by the lower token
  *                                                    (NaN comes last); top_k <= n, up to 64
- * targets and logprobs come together or are both NULL; entropy and stats may be NULL.  stats [rows,3] is opaque, for the
+ * targets and logprobs come together or are both NULL; entropy and stats may be NULL.  inv_temperature may be negative, not
+ * zero.  A NaN or +inf in a row makes its log probabilities and entropy NaN.  n and rows below 2^31.  stats [rows,3] is opaque, for the
  * gradient call.  No counterpart in the reference, which forms all n log probabilities (Tensor/Operators/Unary.swift:198-204). */
 int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t rows, int64_t n, int64_t row_stride,
                                 float inv_temperature, const int32_t *targets, int32_t ignore_index, float *logprobs, float *entropy,

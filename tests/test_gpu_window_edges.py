@@ -225,7 +225,7 @@ def test_training_past_32_bit_offsets(ctx):
 
 @pytest.mark.parametrize("change", [
     dict(H=1 << 15, Hkv=1 << 15, d=256), dict(q_offset=(1 << 30) - 256), dict(Lq=1 << 30), dict(Lk=(1 << 30) - 100),
-    dict(B=1 << 24, Lq=20, Lk=1), dict(B=1 << 29, H=4, Hkv=4)])
+    dict(B=1 << 24, Lq=20, Lk=1), dict(H=4, Lq=1 << 29), dict(H=4, Lq=1 << 29, d=200), dict(B=1 << 29, H=4, Hkv=4)])
 def test_limits_are_refused(ctx, change):
     """Extents that the kernels' 32-bit positions and offsets, or one launch, do not hold."""
     from dl4s_amd import lib
