@@ -176,20 +176,35 @@ int lds_limit(dl4s_hip_ctx *ctx, int family, int kind, K kernel, size_t bytes) {
     return DL4S_HIP_OK;
 }
 
-template <int DT, int BN, bool VEC>
+// Whether eight wavefronts share a workgroup's rows, four to a half of every tile of 64 keys (KS = 2), or four have them alone.
+// They do while a compute unit has no second workgroup to run beside the first, and where there are more than three tiles
+// (d 64, B1 H8 L1024 window 1024, 64 workgroups: forward 46 us with four, 36 with eight, gradients 106 and 89; window 128: 17
+// and 16, 54 and 50; B4 H8 L2048, 512 workgroups: 73 and 81, 285 and 293; d 96, L64: gradients 27 and 28).
+inline bool share_rows(const dl4s_hip_ctx *ctx, const WindowGeometry &g) {
+    return g.units <= ctx->cu_count && std::min<long long>(g.Lk, (long long)g.w.window + g.w.sinks + 128 / g.hp - 1) > 192;
+}
+
+template <int DT, int BN, int KS, bool VEC>
 int launch_fwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, const WindowGeometry &g) {
     typedef Tile<BN, DT> T;
     constexpr size_t lds = 2 * 2 * (T::ROWS_PLANE + T::COLS_PLANE);
-    static_assert(lds <= 65536 - 256, "more LDS needs its limit raised");
-    hipLaunchKernelGGL((sdpa_window_fwd_f32<DT, BN, VEC>), dim3(8 * g.per_xcd), dim3(256), lds, ctx->stream, q, k, v, out, stats, g);
+    const int rc = lds_limit(ctx, dl4s::LDS_WINDOW_FWD, 2 * (DT / 32 - 1) + VEC, sdpa_window_fwd_f32<DT, BN, KS, VEC>, lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((sdpa_window_fwd_f32<DT, BN, KS, VEC>), dim3(8 * g.per_xcd), dim3(256 * KS), lds, ctx->stream, q, k, v, out, stats, g);
     return dl4s::launch_status("sdpa_window_fwd_f32");
 }
 template <bool VEC>
 int launch_fwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *stats, const WindowGeometry &g) {
-    if (g.d <= 32) return launch_fwd<32, 64, VEC>(ctx, q, k, v, out, stats, g);
-    if (g.d <= 64) return launch_fwd<64, 64, VEC>(ctx, q, k, v, out, stats, g);
-    if (g.d <= 96) return launch_fwd<96, 32, VEC>(ctx, q, k, v, out, stats, g);
-    return launch_fwd<128, 32, VEC>(ctx, q, k, v, out, stats, g);
+    if (share_rows(ctx, g)) {
+        if (g.d <= 32) return launch_fwd<32, 64, 2, VEC>(ctx, q, k, v, out, stats, g);
+        if (g.d <= 64) return launch_fwd<64, 64, 2, VEC>(ctx, q, k, v, out, stats, g);
+        if (g.d <= 96) return launch_fwd<96, 64, 2, VEC>(ctx, q, k, v, out, stats, g);
+        return launch_fwd<128, 64, 2, VEC>(ctx, q, k, v, out, stats, g);
+    }
+    if (g.d <= 32) return launch_fwd<32, 64, 1, VEC>(ctx, q, k, v, out, stats, g);
+    if (g.d <= 64) return launch_fwd<64, 64, 1, VEC>(ctx, q, k, v, out, stats, g);
+    if (g.d <= 96) return launch_fwd<96, 32, 1, VEC>(ctx, q, k, v, out, stats, g);
+    return launch_fwd<128, 32, 1, VEC>(ctx, q, k, v, out, stats, g);
 }
 
 // Deals the key blocks to workgroups, of which a compute unit has one at a time.  The blocks without first keys are cut into as
@@ -227,17 +242,28 @@ KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B
     return kb;
 }
 
+template <int DT, int KS, bool VEC>
+int launch_dq(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats, const float *dout,
+              float *dq, float *delta, const WindowGeometry &g) {
+    typedef Tile<32 * KS, DT> T;
+    const size_t lds = 2 * 2 * (2 * T::ROWS_PLANE + T::COLS_PLANE);
+    const int rc = lds_limit(ctx, KS == 2 ? dl4s::LDS_WINDOW_DQ_SHARED : dl4s::LDS_WINDOW_DQ, 2 * (DT / 32 - 1) + VEC, sdpa_window_dq_f32<DT, KS, VEC>, lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((sdpa_window_dq_f32<DT, KS, VEC>), dim3(8 * g.per_xcd), dim3(256 * KS), lds, ctx->stream, q, k, v, out, stats, dout, dq, delta, g);
+    return dl4s::launch_status("sdpa_window_dq_f32");
+}
+
 template <int DT, bool VEC>
 int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats, const float *dout,
                float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
     typedef Tile<32, DT> T;
-    const size_t lds_q = 2 * 2 * (2 * T::ROWS_PLANE + T::COLS_PLANE), lds_k = 2 * 2 * 4 * (T::ROWS_PLANE + T::COLS_PLANE) + 16384;
-    int rc = lds_limit(ctx, dl4s::LDS_WINDOW, 2 * (DT / 32 - 1) + VEC, sdpa_window_dq_f32<DT, VEC>, lds_q);
-    if (!rc) rc = lds_limit(ctx, dl4s::LDS_WINDOW_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dkv_f32<DT, VEC>, lds_k);
+    const size_t lds_k = 2 * 2 * 4 * (T::ROWS_PLANE + T::COLS_PLANE) + 16384;
+    int rc = lds_limit(ctx, dl4s::LDS_WINDOW_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dkv_f32<DT, VEC>, lds_k);
     if (rc) return rc;
     if (g.units) {
-        hipLaunchKernelGGL((sdpa_window_dq_f32<DT, VEC>), dim3(8 * g.per_xcd), dim3(256), lds_q, ctx->stream, q, k, v, out, stats, dout, dq, delta, g);
-        rc = dl4s::launch_status("sdpa_window_dq_f32");
+        // (128 columns: two such wavefronts do not fit the registers of a SIMD)
+        rc = DT <= 96 && share_rows(ctx, g) ? launch_dq<DT, DT <= 96 ? 2 : 1, VEC>(ctx, q, k, v, out, stats, dout, dq, delta, g)
+                                                           : launch_dq<DT, 1, VEC>(ctx, q, k, v, out, stats, dout, dq, delta, g);
         if (rc) return rc;
     }
     if (kb.pairs && kb.blocks) {

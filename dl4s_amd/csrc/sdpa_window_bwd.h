@@ -62,25 +62,26 @@ struct ColumnScale {
     }
 };
 
-template <int DT, bool VEC>
-__global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(const float *__restrict__ q, const float *__restrict__ k,
+template <int DT, int KS, bool VEC>
+__global__ __launch_bounds__(256 * KS, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(const float *__restrict__ q, const float *__restrict__ k,
                                                                             const float *__restrict__ v, const float *__restrict__ out,
                                                                             const float *__restrict__ stats,
                                                                             const float *__restrict__ dout, float *__restrict__ dq,
                                                                             float *__restrict__ delta, const WindowGeometry g) {
-    typedef Tile<32, DT> T;
+    constexpr int BN = 32 * KS;
+    typedef Tile<BN, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
     u16 *Ks = window_lds, *Vs = Ks + 2 * T::ROWS_PLANE, *Kc = Vs + 2 * T::ROWS_PLANE;
-    __shared__ __align__(16) int powers[2][4];             // [K, V]
+    __shared__ __align__(16) int powers[2][BN / 8];        // [K, V]
 
     const int unit = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
     if (unit >= g.units) return;
-    const Place<32> at(g, unit);
-    const int half = (threadIdx.x & 63) >> 5;
+    const Place<BN> at(g, unit);
+    const int half = (threadIdx.x & 63) >> 5, part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
 
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;
-    Stage<32, DT, VEC> kv(ks, g.d, threadIdx.x);
+    Stage<BN, DT, VEC, 256 * KS> kv(ks, g.d, threadIdx.x);
     const int keys = min(at.len, at.wp1 + 1);
     auto load = [&](const int i) {
         const int k0 = at.key0(i);
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
     }, 1.0f));
     del = sum_halves(del);
     const float m = stats[2 * row], inv = stats[2 * row + 1];
-    if (half == 0 && at.qi < g.Lq) delta[row] = del;
+    if (half == 0 && part == 0 && at.qi < g.Lq) delta[row] = del;
     const int p0 = g.w.q_offset + at.q0, p1 = g.w.q_offset + min(at.q0 + 31, g.Lq - 1), p = g.w.q_offset + at.qi;
     const bool idle = at.q0 >= g.Lq;
 
@@ -117,16 +118,16 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
         kv.template store<true, true, true, false>(Ks, Kc, Vs, nullptr, &powers[0][0]);
         __syncthreads();
         if (i + 1 < at.tiles) load(i + 1);
-        const int k0 = at.key0(i);
+        const int k0 = at.key0(i) + 32 * part;
         if (idle || tile_hidden(g.w, p0, p1, k0, at.len)) continue;
         f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
         for (int st = 0; st < DT / 16; ++st)
-            mma3x2(s, T::rows_frag(Ks, 0, st), qf[st], dp, T::rows_frag(Vs, 0, st), gf[st]);
-        const Powers kn(powers[0]);
-        const i32x4 vn = *reinterpret_cast<const i32x4 *>(powers[1]);
+            mma3x2(s, T::rows_frag(Ks, part, st), qf[st], dp, T::rows_frag(Vs, part, st), gf[st]);
+        const Powers kn(&powers[0][4 * part]);
+        const i32x4 vn = *reinterpret_cast<const i32x4 *>(&powers[1][4 * part]);
         settle(s, dp);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -153,15 +154,34 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
             const Frag df = acc_frag(s, st, scale.factor);
             Frag kc[DT / 32];
 #pragma unroll
-            for (int t = 0; t < DT / 32; ++t) kc[t] = T::cols_frag(Kc, t, st);
+            for (int t = 0; t < DT / 32; ++t) kc[t] = T::cols_frag(Kc, t, 2 * part + st);
             mma3(acc, kc, df);
         }
     }
 
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t) settle(acc[t]);
-    if (at.qi >= g.Lq) return;
     const int power = nk - scale.c;
+    f32x4 *sums = reinterpret_cast<f32x4 *>(window_lds);                 // KS = 2: [wavefront][DT / 8][lane], over the tiles
+    const int at_sums = ((threadIdx.x >> 6) & 3) * (DT / 8) * 64 + (threadIdx.x & 63);
+    if (KS == 2) {
+        // the second four wavefronts hand what they have to the first
+        __syncthreads();
+        if (part) {
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = __builtin_ldexpf(acc[t][4 * r + e], power);
+                    sums[at_sums + 64 * (4 * t + r)] = x;
+                }
+        }
+        __syncthreads();
+        if (part) return;
+    }
+    if (at.qi >= g.Lq) return;
     const bool empty = inv == 0.f;                         // saw no key: no gradient, whatever stands in its rows
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t)
@@ -169,7 +189,9 @@ __global__ __launch_bounds__(256, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(cons
         for (int r = 0; r < 4; ++r) {
             f32x4 x = {acc[t][4 * r], acc[t][4 * r + 1], acc[t][4 * r + 2], acc[t][4 * r + 3]};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = __builtin_ldexpf(x[e], power) * g.rT;
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_ldexpf(x[e], power);
+            if (KS == 2) x += sums[at_sums + 64 * (4 * t + r)];
+            x *= g.rT;
             if (empty) x = f32x4{0.f, 0.f, 0.f, 0.f};
             store4(dq + el, 32 * t + 8 * r + 4 * half, g.d, VEC, x);
         }

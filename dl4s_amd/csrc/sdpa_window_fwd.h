@@ -5,6 +5,7 @@
 // all of them and fewer tiles are cut by the window's edges.  Per tile of BN keys:
 //   S^T[key, query] = K . Q^T (K from LDS, Q in registers), mask and online softmax in the accumulators (a lane holds one
 //   query), O^T[column, query] += V^T . P^T with P^T the accumulators themselves as the second operand.
+// In small launches eight wavefronts share the 128 rows, four to a half of the tile's keys (KS = 2), and are merged at the end.
 // Weights carry a factor 2^7, which cancels against their sum: up to 2^15 they fit fp16, and from 2^-14 down they lose bits
 // that are 2^-31 of the row's sum or less.
 // Bound: the matrix instructions (two products of three each), beside which softmax and the splitting into planes run.
@@ -30,7 +31,8 @@ __device__ __forceinline__ bool tile_open(const WindowArgs &w, const int p0, con
     return k0 + 31 <= p0 && k0 + 32 <= len && (k0 > p1 - w.window || k0 + 32 <= w.sinks);
 }
 
-// The workgroup's place: 128 rows of one key head, hp query heads x 128 / hp queries, and the key tiles they see.
+// The workgroup's place: 128 rows of one key head, hp query heads x 128 / hp queries, and the key tiles they see.  Wavefronts
+// 4 .. 7, where there are that many, have the rows of 0 .. 3.
 template <int BN>
 struct Place {
     int qb, part, hk, b, h, rows, q0, qi, qc, len;
@@ -42,7 +44,7 @@ struct Place {
         part = pair % parts;
         hk = pair / parts % g.Hkv;
         b = pair / parts / g.Hkv;
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
         h = hk * g.group + part * g.hp + wave % g.hp;
         rows = 128 / g.hp;
         q0 = qb * rows + wave / g.hp * 32;
@@ -59,8 +61,8 @@ struct Place {
     __device__ __forceinline__ int key0(const int i) const { return (i < first ? i : lo + i - first) * BN; }
 };
 
-template <int DT, int BN, bool VEC>
-__global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(const float *__restrict__ q, const float *__restrict__ k,
+template <int DT, int BN, int KS, bool VEC>
+__global__ __launch_bounds__(256 * KS, DT <= 64 && KS == 1 ? 3 : 2) void sdpa_window_fwd_f32(const float *__restrict__ q, const float *__restrict__ k,
                                                                              const float *__restrict__ v, float *__restrict__ out,
                                                                              float *__restrict__ stats, const WindowGeometry g) {
     typedef Tile<BN, DT> T;
@@ -71,11 +73,11 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
     const int unit = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
     if (unit >= g.units) return;
     const Place<BN> at(g, unit);
-    const int half = (threadIdx.x & 63) >> 5;
+    const int half = (threadIdx.x & 63) >> 5, part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
 
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
     const int ks = (int)g.lk.l, hide0 = g.w.sinks, hide1 = at.wp0 - g.w.window + 1;      // keys between them no query here sees
-    Stage<BN, DT, VEC> kv(ks, g.d, threadIdx.x);
+    Stage<BN, DT, VEC, 256 * KS> kv(ks, g.d, threadIdx.x);
     const int keys = min(at.len, at.wp1 + 1);
     auto load = [&](const int i) {
         const int k0 = at.key0(i);
@@ -105,8 +107,8 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
         if (i + 1 < at.tiles) load(i + 1);
         const int t0 = at.key0(i);
 #pragma unroll
-        for (int sub = 0; sub < BN / 32; ++sub) {
-            const int k0 = t0 + 32 * sub;
+        for (int step = 0; step < BN / 32 / KS; ++step) {
+            const int sub = KS == 1 ? step : BN / 32 / KS * part + step, k0 = t0 + 32 * sub;
             if (idle || tile_hidden(g.w, p0, p1, k0, at.len)) continue;
             f32x16 s;
 #pragma unroll
@@ -162,6 +164,44 @@ __global__ __launch_bounds__(256, DT <= 64 ? 3 : 2) void sdpa_window_fwd_f32(con
 
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t) settle(o[t]);
+    if (KS == 2) {
+        // the second four wavefronts hand what they have to the first
+        f32x4 *sums = reinterpret_cast<f32x4 *>(window_lds);             // [wavefront][DT / 8][lane], over the tiles
+        __shared__ float rest[3][4][64];
+        __shared__ int units[4];
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3, lane = threadIdx.x & 63;
+        __syncthreads();
+        if (part) {
+#pragma unroll
+            for (int t = 0; t < DT / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    sums[(wave * (DT / 8) + 4 * t + r) * 64 + lane] = f32x4{o[t][4 * r], o[t][4 * r + 1], o[t][4 * r + 2], o[t][4 * r + 3]};
+            rest[0][wave][lane] = m_run;
+            rest[1][wave][lane] = m_use;
+            rest[2][wave][lane] = l_run;
+            units[wave] = nv;
+        }
+        __syncthreads();
+        if (part) return;
+        const float m1 = rest[0][wave][lane], u1 = rest[1][wave][lane];
+        const int n1 = __builtin_amdgcn_readfirstlane(units[wave]), n = max(nv, n1);
+        // (what saw no finite score holds zeros, or NaN, which must survive)
+        const float u = m_run == -INFINITY ? (m1 == -INFINITY ? 0.f : u1) : (m1 == -INFINITY ? m_use : fmaxf(m_use, u1));
+        const float f0 = m_run == -INFINITY ? 1.0f : exp2_fast(m_use - u), f1 = m1 == -INFINITY ? 1.0f : exp2_fast(u1 - u);
+        l_run = l_run * f0 + rest[2][wave][lane] * f1;
+        const float g0 = f0 * pow2(max(nv - n, -200)), g1 = f1 * pow2(max(n1 - n, -200));
+#pragma unroll
+        for (int t = 0; t < DT / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const f32x4 x = sums[(wave * (DT / 8) + 4 * t + r) * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[t][4 * r + e] = o[t][4 * r + e] * g0 + x[e] * g1;
+            }
+        m_use = u;
+        nv = n;
+    }
     if (at.qi >= g.Lq) return;
     const float l = sum_halves(l_run);
     // a row that saw no key: zeros

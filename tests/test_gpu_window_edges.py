@@ -270,3 +270,17 @@ def test_limits_of_one_launch(ctx):
         ctx.sdpa_window_fwd(x, x, x, x, None, 1, 1, 1, 1 << 27, 4, 140, 1.0, ctx.window_desc(4))
     assert e.value.code == -5
     x.release()
+
+
+@pytest.mark.parametrize("d", [32, 60, 64, 96, 97, 128])
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk,window,sinks,lengths", [
+    (3, 6, 3, 900, 900, 300, 0, [900, 333, 1]), (1, 16, 4, 700, 700, 700, 7, None), (2, 8, 8, 513, 700, 250, 65, [700, 260]),
+    (1, 9, 9, 500, 500, 1000, 0, [0]), (1, 12, 4, 450, 450, 193, 0, None), (8, 8, 8, 520, 520, 220, 3, None)])
+def test_small_and_large_launches(ctx, B, H, Hkv, Lq, Lk, window, sinks, lengths, d):
+    """Launches of fewer workgroups than compute units, where eight wavefronts share a workgroup's rows, and of more."""
+    rng = np.random.default_rng(Lq + d)
+    q, k, v, g = _inputs(rng, B, H, Hkv, Lq, Lk, d)
+    q[:, :, ::7] *= 8                                      # some rows with one large score, others without
+    rT = float(np.float32(1 / np.sqrt(d)))
+    want = attention(q, k, v, rT, window, sinks, Lk - Lq, lengths, g)
+    _compare(_forward_backward(ctx, q, k, v, g, rT, window, sinks, Lk - Lq, lengths), want, "launches")
