@@ -8,7 +8,11 @@
 // In small launches eight wavefronts share the 128 rows, four to a half of the tile's keys (KS = 2), and are merged at the end.
 // Weights carry a factor 2^7, which cancels against their sum: up to 2^15 they fit fp16, and from 2^-14 down they lose bits
 // that are 2^-31 of the row's sum or less.
-// Bound: the matrix instructions (two products of three each), beside which softmax and the splitting into planes run.
+// Bound: the issue of vector instructions (12 for every matrix instruction) and the matrix instructions (two products of three
+// each) beside them, in turns between barriers.  Measured: B8 H16 L2048 d64 window 512 160 us (190 TFLOP/s on the visible pairs,
+// 157 is the peak of the fp32 instructions; matrix pipe 26 % busy, vector issue about 40 %), B1 H16/4 L8192 d128 window 1024
+// 250 us (260 TFLOP/s, 34 %).  Left out for a timing only: the splitting into planes 27 and 54 us, the softmax 22 and 26, the loads
+// of the next tile 16 and 28.
 #pragma once
 #include "sdpa_window_common.h"
 

@@ -13,6 +13,8 @@
 // workgroup renews it after 1, 2, 4, 8 ... tiles, so about k values per doubling of what has been read come through; each is
 // found by a ballot and inserted by shifting the lanes behind it.  What is left at the end, a few more than k values, is put in
 // order by counting.
+// Measured: 4096 rows of 100000 tokens with 20 alternatives 267 us (6.1 TB/s; without alternatives 250 us = 6.5 TB/s, a plain
+// read of as much reaches 6.6 to 6.9), 2048 rows of 50257 63 us, their gradient 130 us (6.3 TB/s read and written).
 #include "common.h"
 
 #include <algorithm>
@@ -383,13 +385,13 @@ int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t 
                  (long long)top_k, MAX_TOP);
     DL4S_REQUIRE(top_k <= n, DL4S_HIP_ESHAPE, "token_logprobs: %lld alternatives of %lld tokens", (long long)top_k, (long long)n);
     DL4S_REQUIRE(top_k == 0 || (top_logprobs && top_tokens), DL4S_HIP_EINVALID_ARG, "token_logprobs: NULL output for the alternatives");
-    // 16 wavefronts to a row where there are too few rows to fill the GPU with four: up to one row to a compute unit, without
-    // alternatives up to four (with them the renewed bound has 16 wavefronts wait for each other: 1000 rows of 50000 tokens and
-    // 20 alternatives 79 us, with 4 wavefronts 52).  Up to one row to a compute unit long rows come in parts, too, of at least
-    // 16384 tokens (a tile for each wavefront).
-    const bool few = rows <= (top_k ? 1 : 4) * ctx->cu_count;
+    // 16 wavefronts to a row up to one row to a compute unit, otherwise four (256 rows of 50000 tokens 10.9 us and 16.1, with 8
+    // alternatives 19.4 and 29.9; 1000 rows of 5000 tokens 11.1 us and 6.7, with 8 alternatives 27.7 and 13.5: the renewed bound
+    // has the wavefronts wait for each other).  Then long rows come in parts, too, of at least 16384 tokens, a tile for each
+    // wavefront (8 rows of 150000 tokens 9.5 us, in one part 17.2, in parts of 4096 11.9).
+    const bool few = rows <= ctx->cu_count;
     int64_t parts = 1;
-    if (rows <= ctx->cu_count) {
+    if (few) {
         parts = std::min<int64_t>(n / 16384, ctx->cu_count / rows);
         parts = std::min<int64_t>(parts, top_k ? MERGE_KEYS / top_k : 64);
         parts = std::max<int64_t>(parts, 1);
