@@ -269,3 +269,25 @@ def test_temperatures_of_the_log_probabilities(ctx, t):
     assert np.abs(bufs[2].numpy() - lp[np.arange(rows), targets]).max() <= bound
     for b in bufs:
         b.release()
+
+
+@pytest.mark.parametrize("rows,n", [(70000, 5), (131071, 3)])
+def test_more_rows_than_a_grid_axis(ctx, rows, n):
+    """Log probabilities and their gradient: the rows behind the 65535th are like the first ones, which are checked elsewhere."""
+    rng = np.random.default_rng(26)
+    first = 50
+    x = np.resize(_f32(rng, first, n), (rows, n))
+    targets, up = np.resize(rng.integers(0, n, first), rows), np.resize(_f32(rng, first), rows)
+    got = []
+    for m in (first, rows):
+        bufs = [ctx.to_device(x[:m]), ctx.to_device(targets[:m], np.int32), ctx.to_device(up[:m])]
+        outs = [ctx.empty((m,)), ctx.empty((m,)), ctx.empty((m, 3)), ctx.empty((m, 2)), ctx.empty((m, 2), np.int32), ctx.empty((m, n))]
+        ctx.token_logprobs(bufs[0], m, n, n, bufs[1], outs[0], entropy=outs[1], stats=outs[2], top_k=2, top_logprobs=outs[3], top_tokens=outs[4])
+        ctx.token_logprobs_bwd(bufs[0], m, n, n, bufs[1], outs[2], outs[5], dlogprobs=bufs[2], dentropy=bufs[2])
+        got.append([o.numpy() for o in outs])
+        for b in bufs + outs:
+            b.release()
+    # 16 wavefronts to a row for few rows, four for many: both end with the same one value a lane, in other lanes
+    for a, b in zip(*got):
+        a = np.resize(a, b.shape)
+        assert np.array_equal(a, b) if a.dtype == np.int32 else np.abs(a - b).max() <= 2.0 ** -24 * 64 * (1 + np.abs(a).max())
