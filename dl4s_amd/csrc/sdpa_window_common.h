@@ -100,21 +100,26 @@ __device__ __forceinline__ int coarse_scale_of(const float m) {
 constexpr int MOST_POWER = 123;                            // the largest of these
 __device__ __forceinline__ float finite_abs(const float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
 template <int CTRL>
-__device__ __forceinline__ float max_lanes(const float v) {
-    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)));
+__device__ __forceinline__ unsigned max_lanes(const unsigned u) {
+    return max(u, (unsigned)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xF, 0xF, true));
 }
-// Largest of the 64 lanes' values (>= 0), uniform.
-__device__ __forceinline__ float wave_max_abs(float v) {
-    v = max_lanes<0xB1>(v);
-    v = max_lanes<0x4E>(v);
-    v = max_lanes<0x141>(v);
-    v = max_lanes<0x140>(v);
-    const unsigned u = __float_as_uint(v);
+// Largest of the 64 lanes' values (>= 0, so their bits are in the same order), uniform.
+__device__ __forceinline__ float wave_max_abs(const float v) {
+    unsigned u = __float_as_uint(v);
+    u = max_lanes<0xB1>(u);
+    u = max_lanes<0x4E>(u);
+    u = max_lanes<0x141>(u);
+    u = max_lanes<0x140>(u);
     const unsigned r0 = __builtin_amdgcn_readlane(u, 0), r1 = __builtin_amdgcn_readlane(u, 16), r2 = __builtin_amdgcn_readlane(u, 32),
                    r3 = __builtin_amdgcn_readlane(u, 48);
     return __uint_as_float(max(max(r0, r1), max(r2, r3)));
 }
-// max(m, |a|, |b|) without the quieting of signalling NaNs that fmaxf brings along (a NaN is passed over)
+// Maxima without the quieting of signalling NaNs that fmaxf brings along (a NaN is passed over)
+__device__ __forceinline__ float max3(const float a, const float b, const float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 __device__ __forceinline__ float max_abs(const float m, const float a, const float b) {
     float r;
     asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(m), "v"(a), "v"(b));

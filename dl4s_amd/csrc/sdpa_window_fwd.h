@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256 * KS, DT <= 64 && KS == 1 ? 3 : 2) void sdpa_wi
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 f[x] = fmaxf(__builtin_ldexpf(unq, nk[x]), 1.17549435e-38f);
-                tmax = fmaxf(tmax, fmaxf(fmaxf(s[4 * x], s[4 * x + 1]), fmaxf(s[4 * x + 2], s[4 * x + 3])) * f[x]);
+                tmax = fmaxf(tmax, max3(max3(s[4 * x], s[4 * x + 1], s[4 * x + 2]), s[4 * x + 3], s[4 * x + 3]) * f[x]);
             }
             // the reference maximum moves, and the sums are rescaled, only when a weight would pass 2^8 (x 2^7): any factor
             // left in the weights of a row cancels in the division by their sum

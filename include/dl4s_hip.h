@@ -304,8 +304,8 @@ int dl4s_hip_argmax_to_f32(dl4s_hip_ctx *ctx, const float *values, int64_t count
  * infinity is NaN there too.  An infinity among the operands of a visible pair gives NaN.
  * Precision: fp32 throughout; up to 128 columns the products are formed from two fp16 halves of each operand that share a
  * power of two along a row, or among the rows of k, v, q, dout that are read together, so a value also carries an error of up
- * to 2^-36 of the largest of those rows, a weight one of up to 2^-32 (sums of 64 products of like-sized values are off by 1.2e-7, 1.5e-7
- * on the fp32 instructions).
+ * to 2^-36 of the largest of those rows, a weight one of up to 2^-32 (sums of 64 products of like-sized values are off by 1.2e-7 of
+ * their size, 1.5e-7 on the fp32 instructions).
  * Limits (DL4S_HIP_EUNSUPPORTED): H * d up to 2^22, q_offset + Lq and Lk up to 2^30 - 256, B * H below 2^30, fewer than 2^32 rows,
  * and 2^24 workgroups of a launch (of 128 rows, above 128 columns of 4; half as many of 16 for few rows).  The first call of a
  * shape may need the library's scratch block to grow, which a recording refuses: run the same call once before. */
