@@ -7,7 +7,7 @@
 //     group.  Two wavefronts share 32 keys (the columns of their accumulators): one holds K and forms S = Q . K^T, the weights
 //     w, and dV^T += dO^T . w, the other holds V and forms dP = dO . V^T and, with the weights it gets through LDS,
 //     dK^T += Q^T . dS.  That halves what a wavefront keeps in registers, so two run on a SIMD at every head dim (one
-//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes 395 us at B2 H16/4 L4096 d96 window 777).
+//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes 392 us at B2 H16/4 L4096 d96 window 777).
 //     Shared key heads are summed in the accumulators, in a fixed order, without atomics.  Key blocks that hold visible
 //     first keys are seen by every later query: their query tiles are dealt to several workgroups whose partial sums a
 //     last kernel adds up in order; so are all blocks where that shortens the longest queue of a compute unit.
@@ -16,7 +16,7 @@
 // later one would pass 2^15.
 // Seven products for the five of the gradient, each three matrix instructions per 16-deep step, and the vector instructions of
 // the splitting, which every tile goes through in both forms, rows and columns: their issue bounds both kernels (B2 H16/4 L4096
-// d96 window 777: dq 229 us with the matrix pipe 32 % busy, dk/dv 395 us, 23 %).
+// d96 window 777: dq 229 us with the matrix pipe 32 % busy, dk/dv 392 us, 23 %).
 #pragma once
 #include "sdpa_window_fwd.h"
 
@@ -227,8 +227,7 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
     extern __shared__ __align__(16) u16 window_lds[];
     constexpr int BUF = 4 * (T::ROWS_PLANE + T::COLS_PLANE);     // [Q rows][dO rows][Q columns][dO columns]
     f32x4 *weights = reinterpret_cast<f32x4 *>(window_lds + 2 * BUF);      // [pair of wavefronts][4][lane]
-    __shared__ __align__(16) float row_values[2][64];      // [buffer][2][32] of the tile's queries: m + log2(l) - 13 (a rounding of
-                                                           // 2^-24 of it: less than the scores it is taken from have), delta
+    __shared__ __align__(16) float row_values[2][96];      // [buffer][3][32]: m, 2^13 / l, delta of the tile's queries
     __shared__ __align__(16) int powers[2][2][4];          // [buffer][Q, dO]
 
     int id = blockIdx.x, cl = 1;
@@ -263,10 +262,11 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
     auto load = [&]() {
         const int r0 = next * 32;
         qg.load(qp, gp, qs, r0, rows - r0, g.d);
-        if (threadIdx.x < 64) {
-            const int r = r0 + (threadIdx.x & 31);
-            sv = threadIdx.x < 32 ? INFINITY : 0.f;
-            if (r < rows) sv = threadIdx.x < 32 ? stats[2 * (row0 + r)] - log2f(stats[2 * (row0 + r) + 1]) - 13.0f : delta[row0 + r];
+        if (threadIdx.x < 96) {
+            const int which = threadIdx.x >> 5, r = r0 + (threadIdx.x & 31);
+            sv = 0.f;
+            if (r < rows) sv = which == 2 ? delta[row0 + r] : stats[2 * (row0 + r) + which];
+            if (which == 1) sv *= 8192.0f;
         }
         if (++next == t1) {                                // on to the group's next head
             next = t0;
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
         const int buf = (e - from) & 1;
         u16 *Qs = window_lds + buf * BUF, *Gs = Qs + 2 * T::ROWS_PLANE, *Qc = Gs + 2 * T::ROWS_PLANE, *Gc = Qc + 2 * T::COLS_PLANE;
         qg.template store<true, true, true, true>(Qs, Qc, Gs, Gc, &powers[buf][0][0], g.rT * LOG2E);
-        if (threadIdx.x < 64) row_values[buf][threadIdx.x] = sv;
+        if (threadIdx.x < 96) row_values[buf][threadIdx.x] = sv;
         if (e + 1 < to) load();
     };
     int now = next;                                        // the tile that is worked on
@@ -330,13 +330,17 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const float f = __builtin_ldexpf(unscale, n[x]);
-                const f32x4 m = *reinterpret_cast<const f32x4 *>(rowv + (values ? 32 : 0) + 8 * x + 4 * half);
+                const f32x4 m = *reinterpret_cast<const f32x4 *>(rowv + (values ? 64 : 0) + 8 * x + 4 * half);
 #pragma unroll
-                for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_fmaf(s[4 * x + y], f, -m[y]);     // log2(2^13 w), or dP - delta
+                for (int y = 0; y < 4; ++y) s[4 * x + y] = __builtin_fmaf(s[4 * x + y], f, -m[y]);     // s - m, or dP - delta
             }
             if (!values) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = exp2_fast(s[r]);
+                for (int x = 0; x < 4; ++x) {
+                    const f32x4 inv = *reinterpret_cast<const f32x4 *>(rowv + 32 + 8 * x + 4 * half);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) s[4 * x + y] = exp2_fast(s[4 * x + y]) * inv[y];
+                }
                 if (!open) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
