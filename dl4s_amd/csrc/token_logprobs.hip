@@ -29,6 +29,11 @@ typedef unsigned long long u64;
 
 __device__ __forceinline__ float scaled(const float x, const float t) { return x * t + 0.0f; }   // + 0: the two zeros are one value
 __device__ __forceinline__ float exp_fast(const float y) { return __builtin_amdgcn_exp2f(y * LOG2E); }
+// With what the change of base rounds off put back (|y| <= 1e4): a far y's exponential is off by a step, not by |y| steps.
+__device__ __forceinline__ float exp_near(const float y) {
+    const float t = y * LOG2E, r = __builtin_fmaf(y, 1.925963033500702e-8f, __builtin_fmaf(y, LOG2E, -t));
+    return __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, 0.69314718055994530942f, 1.0f);
+}
 
 // The order of the alternatives as one integer: larger value first, of equal values the lower token; NaN behind -inf.  0 is no token.
 __device__ __forceinline__ u64 order_key(const float z, const unsigned token) {
@@ -87,7 +92,7 @@ __device__ __forceinline__ void row_results(const Outputs &o, const long long ro
         o.logprobs[row] = g == o.ignore ? 0.f : (g < 0 || g >= n ? __builtin_nanf("") : (scaled(xr[g], t) - s.m) - L);
     }
     if (o.entropy) o.entropy[row] = H;
-    if (o.stats) { o.stats[3 * row] = s.m; o.stats[3 * row + 1] = L; o.stats[3 * row + 2] = H; }
+    if (o.stats) { o.stats[3 * row] = s.m; o.stats[3 * row + 1] = s.l; o.stats[3 * row + 2] = H; }
 }
 // The `top` largest of `count` keys in LDS (0 = none) as outputs, or as keys: each is put where its rank says.  The keys are
 // read in pieces of eight: the list is filled up with zeros.
@@ -313,15 +318,17 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_f32(const float *x, co
                                                                const float *__restrict__ stats, const float *__restrict__ dlogprobs,
                                                                const float *__restrict__ dentropy, float *dx) {
     const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
-    const float m = stats[3 * row], L = stats[3 * row + 1], H = stats[3 * row + 2];
+    const float m = stats[3 * row], l = stats[3 * row + 1], H = stats[3 * row + 2], L = logf(l), inv = 1.0f / l;
     const int g = targets ? targets[row] : ignore;
     const float gl = (dlogprobs && g != ignore) ? (g < 0 || g >= n ? __builtin_nanf("") : dlogprobs[row]) : 0.f;
     const float ge = dentropy ? dentropy[row] : 0.f;
     const float *xr = x + row * stride;
     float *dr = dx + row * stride;
     auto gradient = [&](const float v, const long long j) {
-        const float lp = (scaled(v, t) - m) - L, p = exp_fast(lp);
-        float r = -p * (gl + ge * (fmaxf(lp, -1e4f) + H));
+        float y = scaled(v, t) - m;
+        y = y < -1e4f ? -1e4f : y;                                     // (a NaN stays)
+        // (not from log p: the subtraction of L rounds by as much as a far z)
+        float r = -(exp_near(y) * inv) * (gl + ge * ((y - L) + H));
         if (j == g) r += gl;
         return r * t;
     };
