@@ -211,19 +211,20 @@ int launch_fwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const fl
 // many pieces as make the longest queue of a compute unit shortest (in query tiles: a workgroup costs about one more, a
 // second launch that adds up partial sums about three, and their way through memory); those with first keys, which
 // every later query sees, into enough pieces to give every compute unit one.  At most 2048 workgroups leave partial sums.
-KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B) {
+// beside: the workgroups share the GPU with those of dq; they are to be no more than the compute units that those leave.
+KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B, bool beside) {
     KeyBlocks kb;
     kb.pairs = (int)(B * g.Hkv);
     kb.blocks = (g.Lk + 127) / 128;
     kb.sink_blocks = std::min(kb.blocks, (g.w.sinks + 127) / 128);
-    const long long cus = ctx->cu_count, tiles = (g.Lq + 31) / 32, near = std::min<long long>(tiles, (g.w.window + 127ll + 31) / 32 + 1);
+    const long long cus = ctx->cu_count - (beside ? g.units : 0), tiles = (g.Lq + 31) / 32, near = std::min<long long>(tiles, (g.w.window + 127ll + 31) / 32 + 1);
     const long long n[2] = {tiles * g.group, near * g.group}, count[2] = {(long long)kb.pairs * kb.sink_blocks, (long long)kb.pairs * (kb.blocks - kb.sink_blocks)};
-    long long floats = 0;
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 1; c >= 0; --c) {
         const long long most = std::max(1ll, std::min(n[c] / 4, 2048 / std::max(1ll, count[c])));
         long long chunks = 1;
         if (c == 0) {
-            chunks = std::min(most, std::max(1ll, (cus + count[0] - 1) / std::max(1ll, count[0])));
+            const long long left = beside ? cus - kb.units[1] : cus + count[0] - 1;
+            chunks = std::min(most, std::max(1ll, left / std::max(1ll, count[0])));
         } else {
             double best = 0;
             for (long long x = 1; x <= std::min(most, 8ll); ++x) {
@@ -235,10 +236,10 @@ KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B
         kb.chunks[c] = (int)chunks;
         kb.units[c] = (int)(count[c] * chunks);
         kb.per_xcd[c] = (kb.units[c] + 7) / 8;
-        if (c) kb.class1 = floats;
-        if (chunks > 1) floats += count[c] * chunks * 256 * g.d;
     }
-    kb.partial = reinterpret_cast<float *>(floats * sizeof(float));      // the caller replaces the size by the address
+    const long long floats0 = kb.chunks[0] > 1 ? kb.units[0] * 256ll * g.d : 0, floats1 = kb.chunks[1] > 1 ? kb.units[1] * 256ll * g.d : 0;
+    kb.class1 = floats0;
+    kb.partial = reinterpret_cast<float *>((floats0 + floats1) * sizeof(float));      // the caller replaces the size by the address
     return kb;
 }
 
@@ -255,21 +256,37 @@ int launch_dq(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v,
 
 template <int DT, bool VEC>
 int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats, const float *dout,
-               float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
+               float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb, const bool beside) {
     typedef Tile<32, DT> T;
     const size_t lds_k = 2 * 2 * 4 * (T::ROWS_PLANE + T::COLS_PLANE) + 16384;
-    int rc = lds_limit(ctx, dl4s::LDS_WINDOW_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dkv_f32<DT, VEC>, lds_k);
+    int rc = DL4S_HIP_OK;
+    if constexpr (DT <= 96) {
+        typedef Tile<64, DT> T2;
+        if (beside) {
+            const size_t lds = std::max(lds_k, (size_t)(2 * 2 * (2 * T2::ROWS_PLANE + T2::COLS_PLANE)));
+            rc = lds_limit(ctx, dl4s::LDS_WINDOW_DQ_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dq_dkv_f32<DT, VEC>, lds);
+            if (rc) return rc;
+            const long long rows = (long long)kb.pairs * g.group * g.Lq;
+            hipLaunchKernelGGL(window_delta_f32, row_grid(rows), dim3(256), 0, ctx->stream, dout, out, delta, g.H, g.Lq, g.d, g.lq, rows);
+            hipLaunchKernelGGL((sdpa_window_dq_dkv_f32<DT, VEC>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1] + g.per_xcd)), dim3(512), lds, ctx->stream,
+                               q, k, v, out, stats, dout, delta, dq, dk, dv, g, kb);
+            rc = dl4s::launch_status("sdpa_window_dq_dkv_f32");
+        }
+    }
+    if (!rc && !beside) rc = lds_limit(ctx, dl4s::LDS_WINDOW_DKV, 2 * (DT / 32 - 1) + VEC, sdpa_window_dkv_f32<DT, VEC>, lds_k);
     if (rc) return rc;
-    if (g.units) {
+    if (!beside && g.units) {
         // (128 columns: two such wavefronts do not fit the registers of a SIMD)
         rc = DT <= 96 && share_rows(ctx, g) ? launch_dq<DT, DT <= 96 ? 2 : 1, VEC>(ctx, q, k, v, out, stats, dout, dq, delta, g)
                                                            : launch_dq<DT, 1, VEC>(ctx, q, k, v, out, stats, dout, dq, delta, g);
         if (rc) return rc;
     }
     if (kb.pairs && kb.blocks) {
-        hipLaunchKernelGGL((sdpa_window_dkv_f32<DT, VEC>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1])), dim3(512), lds_k, ctx->stream, q, k, v, stats,
-                           dout, delta, dk, dv, g, kb);
-        rc = dl4s::launch_status("sdpa_window_dkv_f32");
+        if (!beside) {
+            hipLaunchKernelGGL((sdpa_window_dkv_f32<DT, VEC>), dim3(8 * (kb.per_xcd[0] + kb.per_xcd[1])), dim3(512), lds_k, ctx->stream, q, k, v, stats,
+                               dout, delta, dk, dv, g, kb);
+            rc = dl4s::launch_status("sdpa_window_dkv_f32");
+        }
         for (int c = 0; c < 2 && !rc; ++c) {
             const int first = c ? kb.sink_blocks : 0, n = c ? kb.blocks - kb.sink_blocks : kb.sink_blocks;
             if (kb.chunks[c] == 1 || n == 0) continue;
@@ -282,11 +299,12 @@ int launch_bwd(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v
 
 template <bool VEC>
 int launch_bwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out, const float *stats,
-                     const float *dout, float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb) {
-    if (g.d <= 32) return launch_bwd<32, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
-    if (g.d <= 64) return launch_bwd<64, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
-    if (g.d <= 96) return launch_bwd<96, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
-    return launch_bwd<128, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+                     const float *dout, float *dq, float *dk, float *dv, float *delta, const WindowGeometry &g, const KeyBlocks &kb,
+                     const bool beside) {
+    if (g.d <= 32) return launch_bwd<32, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb, beside);
+    if (g.d <= 64) return launch_bwd<64, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb, beside);
+    if (g.d <= 96) return launch_bwd<96, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb, beside);
+    return launch_bwd<128, VEC>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb, beside);
 }
 
 // Few query rows: the workgroups and the split of the keys.  Lk is the number of rows that can be visible at all (T of a cache).
@@ -419,7 +437,15 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
     const size_t delta_bytes = ((size_t)rows * sizeof(float) + 255) / 256 * 256;
     if (d <= 128 && H > 0) {
         const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
-        KeyBlocks kb = krows ? key_blocks(ctx, g, B) : KeyBlocks{};
+        // dq and dk/dv run side by side, behind a small kernel for delta, where all their workgroups find a compute unit of
+        // their own (d 64, one after the other and side by side: B4 H8 L512 window 128 50 us and 33, B1 H8 L2048 window 1024 117
+        // and 94, L64 21 and 13; d 96: 67 and 42, 153 and 117, 26 and 16); above 96 columns dq needs a SIMD's registers alone
+        bool beside = d <= 96 && rows && krows && 2 * g.units <= ctx->cu_count;
+        KeyBlocks kb = krows ? key_blocks(ctx, g, B, beside) : KeyBlocks{};
+        if (beside && g.units + kb.units[0] + kb.units[1] > ctx->cu_count) {
+            beside = false;
+            kb = key_blocks(ctx, g, B, false);
+        }
         rc = fits_a_launch("sdpa_window_bwd", std::max(8ll * g.per_xcd, 16ll * (kb.per_xcd[0] + kb.per_xcd[1])), 256);
         if (rc) return rc;
         rc = dl4s::ensure_scratch(ctx, delta_bytes + reinterpret_cast<size_t>(kb.partial));
@@ -427,8 +453,8 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
         float *delta = reinterpret_cast<float *>(ctx->scratch);
         kb.partial = delta + delta_bytes / sizeof(float);
         return d % 4 == 0 && on_16_bytes({q, k, v, out, dout, dq, dk, dv})
-                   ? launch_bwd_width<true>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb)
-                   : launch_bwd_width<false>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb);
+                   ? launch_bwd_width<true>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb, beside)
+                   : launch_bwd_width<false>(ctx, q, k, v, out, stats, dout, dq, dk, dv, delta, g, kb, beside);
     }
     rc = fits_a_launch("sdpa_window_bwd", std::max(rows + 3, krows + 3) / 4, 256);
     if (!rc) rc = dl4s::ensure_scratch(ctx, delta_bytes);

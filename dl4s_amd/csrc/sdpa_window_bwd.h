@@ -64,19 +64,19 @@ struct ColumnScale {
     }
 };
 
+// (delta may be NULL: another kernel has formed it)
 template <int DT, int KS, bool VEC>
-__global__ __launch_bounds__(256 * KS, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(const float *__restrict__ q, const float *__restrict__ k,
-                                                                            const float *__restrict__ v, const float *__restrict__ out,
-                                                                            const float *__restrict__ stats,
-                                                                            const float *__restrict__ dout, float *__restrict__ dq,
-                                                                            float *__restrict__ delta, const WindowGeometry g) {
+__device__ __forceinline__ void window_dq(const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
+                                          const float *__restrict__ out, const float *__restrict__ stats,
+                                          const float *__restrict__ dout, float *__restrict__ dq, float *__restrict__ delta,
+                                          const WindowGeometry &g, const int workgroup) {
     constexpr int BN = 32 * KS;
     typedef Tile<BN, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
     u16 *Ks = window_lds, *Vs = Ks + 2 * T::ROWS_PLANE, *Kc = Vs + 2 * T::ROWS_PLANE;
     __shared__ __align__(16) int powers[2][BN / 8];        // [K, V]
 
-    const int unit = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
+    const int unit = (workgroup & 7) * g.per_xcd + (workgroup >> 3);
     if (unit >= g.units) return;
     const Place<BN> at(g, unit);
     const int half = (threadIdx.x & 63) >> 5, part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256 * KS, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32
     }, 1.0f));
     del = sum_halves(del);
     const float m = stats[2 * row], inv = stats[2 * row + 1];
-    if (half == 0 && part == 0 && at.qi < g.Lq) delta[row] = del;
+    if (delta && half == 0 && part == 0 && at.qi < g.Lq) delta[row] = del;
     const int p0 = g.w.q_offset + at.q0, p1 = g.w.q_offset + min(at.q0 + 31, g.Lq - 1), p = g.w.q_offset + at.qi;
     const bool idle = at.q0 >= g.Lq;
 
@@ -199,6 +199,15 @@ __global__ __launch_bounds__(256 * KS, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32
         }
 }
 
+template <int DT, int KS, bool VEC>
+__global__ __launch_bounds__(256 * KS, DT <= 96 ? 2 : 1) void sdpa_window_dq_f32(const float *__restrict__ q, const float *__restrict__ k,
+                                                                                 const float *__restrict__ v, const float *__restrict__ out,
+                                                                                 const float *__restrict__ stats,
+                                                                                 const float *__restrict__ dout, float *__restrict__ dq,
+                                                                                 float *__restrict__ delta, const WindowGeometry g) {
+    window_dq<DT, KS, VEC>(q, k, v, out, stats, dout, dq, delta, g, blockIdx.x);
+}
+
 // How the key blocks (128 keys) of all (batch, key head) pairs are dealt to workgroups: class 0 are those that hold visible
 // first keys, class 1 the others; each in `chunks` equal pieces of its query tiles.  The pieces of class 1 are started
 // first, the shorter ones of class 0 fill up.  Workgroup ids of a class go round the XCDs so that consecutive pieces of
@@ -218,11 +227,10 @@ __device__ __forceinline__ float *partial_sums(const KeyBlocks &kb, const int pa
 }
 
 template <int DT, bool VEC>
-__global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__restrict__ q, const float *__restrict__ k,
-                                                               const float *__restrict__ v, const float *__restrict__ stats,
-                                                               const float *__restrict__ dout, const float *__restrict__ delta,
-                                                               float *__restrict__ dk, float *__restrict__ dv, const WindowGeometry g,
-                                                               const KeyBlocks kb) {
+__device__ __forceinline__ void window_dkv(const float *__restrict__ q, const float *__restrict__ k, const float *__restrict__ v,
+                                           const float *__restrict__ stats, const float *__restrict__ dout,
+                                           const float *__restrict__ delta, float *__restrict__ dk, float *__restrict__ dv,
+                                           const WindowGeometry &g, const KeyBlocks &kb, const int workgroup) {
     typedef Tile<32, DT> T;
     extern __shared__ __align__(16) u16 window_lds[];
     constexpr int BUF = 4 * (T::ROWS_PLANE + T::COLS_PLANE);     // [Q rows][dO rows][Q columns][dO columns]
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
     __shared__ __align__(16) float row_values[2][96];      // [buffer][3][32]: m, 2^13 / l, delta of the tile's queries
     __shared__ __align__(16) int powers[2][2][4];          // [buffer][Q, dO]
 
-    int id = blockIdx.x, cl = 1;
+    int id = workgroup, cl = 1;
     if (id >= 8 * kb.per_xcd[1]) { id -= 8 * kb.per_xcd[1]; cl = 0; }
     const int unit = (id & 7) * kb.per_xcd[cl] + (id >> 3);
     if (unit >= kb.units[cl]) return;
@@ -408,6 +416,29 @@ __global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__res
             for (int e = 0; e < 4; ++e) x[e] = __builtin_ldexpf(x[e] * factor_out, power);
             store4(to_row, 32 * t + 8 * r + 4 * half, g.d, VEC, x);
         }
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(512, 2) void sdpa_window_dkv_f32(const float *__restrict__ q, const float *__restrict__ k,
+                                                              const float *__restrict__ v, const float *__restrict__ stats,
+                                                              const float *__restrict__ dout, const float *__restrict__ delta,
+                                                              float *__restrict__ dk, float *__restrict__ dv, const WindowGeometry g,
+                                                              const KeyBlocks kb) {
+    window_dkv<DT, VEC>(q, k, v, stats, dout, delta, dk, dv, g, kb, blockIdx.x);
+}
+
+// Both at once, where all their workgroups find a compute unit of their own: side by side they take as long as the longer one.
+// delta has been formed before.
+template <int DT, bool VEC>
+__global__ __launch_bounds__(512, 2) void sdpa_window_dq_dkv_f32(const float *__restrict__ q, const float *__restrict__ k,
+                                                                 const float *__restrict__ v, const float *__restrict__ out,
+                                                                 const float *__restrict__ stats, const float *__restrict__ dout,
+                                                                 const float *__restrict__ delta, float *__restrict__ dq,
+                                                                 float *__restrict__ dk, float *__restrict__ dv, const WindowGeometry g,
+                                                                 const KeyBlocks kb) {
+    const int first = 8 * (kb.per_xcd[0] + kb.per_xcd[1]), workgroup = blockIdx.x;
+    if (workgroup < first) window_dkv<DT, VEC>(q, k, v, stats, dout, delta, dk, dv, g, kb, workgroup);
+    else window_dq<DT, 2, VEC>(q, k, v, out, stats, dout, dq, nullptr, g, workgroup - first);
 }
 
 // Adds up the partial sums of the key blocks that were dealt to several workgroups, chunk after chunk.  One thread per
