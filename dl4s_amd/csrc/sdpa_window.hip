@@ -439,7 +439,8 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
         const WindowGeometry g = geometry(B, H, Hkv, Lq, Lk, d, inv_temperature, tm, w);
         // dq and dk/dv run side by side, behind a small kernel for delta, where all their workgroups find a compute unit of
         // their own (d 64, one after the other and side by side: B4 H8 L512 window 128 50 us and 33, B1 H8 L2048 window 1024 117
-        // and 94, L64 21 and 13; d 96: 67 and 42, 153 and 117, 26 and 16); above 96 columns dq needs a SIMD's registers alone
+        // and 94, L64 21 and 13; d 96: 67 and 42, 153 and 117, 26 and 16; with two workgroups to a compute unit, B4 H8 L1024
+        // window 128, 53 and 57); above 96 columns dq needs a SIMD's registers alone
         bool beside = d <= 96 && rows && krows && 2 * g.units <= ctx->cu_count;
         KeyBlocks kb = krows ? key_blocks(ctx, g, B, beside) : KeyBlocks{};
         if (beside && g.units + kb.units[0] + kb.units[1] > ctx->cu_count) {
