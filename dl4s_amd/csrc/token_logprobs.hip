@@ -318,10 +318,11 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_f32(const float *x, co
                                                                const float *__restrict__ stats, const float *__restrict__ dlogprobs,
                                                                const float *__restrict__ dentropy, float *dx) {
     const long long row = blockIdx.y + (long long)blockIdx.z * 65535;
-    const float m = stats[3 * row], l = stats[3 * row + 1], H = stats[3 * row + 2], L = logf(l), inv = 1.0f / l;
+    const float m = stats[3 * row], l = stats[3 * row + 1], L = logf(l), inv = 1.0f / l;
     const int g = targets ? targets[row] : ignore;
     const float gl = (dlogprobs && g != ignore) ? (g < 0 || g >= n ? __builtin_nanf("") : dlogprobs[row]) : 0.f;
-    const float ge = dentropy ? dentropy[row] : 0.f;
+    // (the entropy enters only where it has a gradient: zero times what may stand there is not always zero)
+    const float ge = dentropy ? dentropy[row] : 0.f, H = ge == 0.f ? 0.f : stats[3 * row + 2];
     const float *xr = x + row * stride;
     float *dr = dx + row * stride;
     auto gradient = [&](const float v, const long long j) {
