@@ -62,8 +62,10 @@ __device__ __forceinline__ u64 key_before(const u64 key) {       // the key of t
 struct Sums {
     float m, l, u;
 };
-__device__ __forceinline__ Sums rescaled(const Sums s, const float M) {      // s with M in place of its maximum
-    const float f = s.m == -INFINITY ? 0.f : exp_fast(s.m - M), d = s.m == -INFINITY ? 0.f : s.m - M;
+// s with M in place of its maximum.  Far below M the weight f is zero, and the distance is held at -1e4 as it is for a token's value:
+// a masked value's distance times the number of such values is past fp32's range (where it is NaN, so is f).
+__device__ __forceinline__ Sums rescaled(const Sums s, const float M) {
+    const float f = s.m == -INFINITY ? 0.f : exp_fast(s.m - M), d = s.m == -INFINITY ? 0.f : fmaxf(s.m - M, -1e4f);
     Sums r;
     r.m = M;
     r.l = s.m == -INFINITY ? s.l : s.l * f;

@@ -74,3 +74,29 @@ def test_gradient_without_the_entropy(ctx, mask, rows, n):
         _close(_gradient(ctx, x, 1.0, targets, -1, g, spoil=spoil), d, bound, "gradient")
     # an upstream gradient of zero for the entropies is the same as none
     _close(_gradient(ctx, x, 1.0, targets, -1, g, h=np.zeros(rows)), d, bound, "gradient, entropies' zero")
+
+
+@pytest.mark.parametrize("rows,n", SHAPES)
+@pytest.mark.parametrize("top", [0, 20])
+@pytest.mark.parametrize("mask", [LOWEST, -1e38, -1e37, -1e36, -1e9])
+def test_entropies_of_masked_rows(ctx, mask, top, rows, n):
+    """A lane, a wavefront or a part of a row may meet nothing but masked tokens: their distance to the row's maximum, times
+    their number, is past fp32's range where their weight is zero."""
+    rng = np.random.default_rng(n + top)
+    for live, t in ((8, 1.0), (1, 0.7)):
+        x, targets = _masked(rng, rows, n, mask, live)
+        _check(ctx, x, n, t=t, targets=targets, top=top, grads=True, what="mask %g, %d live" % (mask, live))
+    x, targets = _masked(rng, rows, n, mask, n // 2)
+    _check(ctx, x, n, targets=targets, top=top, grads=True, what="mask %g, half" % mask)
+
+
+@pytest.mark.parametrize("n", [700, 40000])
+def test_logits_from_end_to_end_of_the_range(ctx, n):
+    """Rows whose logits rise or fall over the whole range of fp32, and rows of nothing but its lowest value."""
+    x = np.empty((4, n), np.float32)
+    x[0] = np.linspace(LOWEST, -LOWEST, n)
+    x[1] = x[0, ::-1]
+    x[2] = LOWEST
+    x[3] = np.where(np.arange(n) % 2, LOWEST, 0.0)
+    for top in (0, 7):
+        _check(ctx, x, n, targets=np.array([n - 1, 0, n // 2, 2]), top=top, grads=True, what="range")

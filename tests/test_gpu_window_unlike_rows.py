@@ -1,0 +1,62 @@
+"""Windowed attention of tensors whose rows differ in size by more than 2^13: a row that is read long after, or in another head than,
+a larger one is as exact as if that one were not there.
+
+The outputs compared are those that no large row enters.  Their exact values are the same with the large rows replaced by zeros, and
+the bounds (window_reference) are those of the tensors with the large rows replaced: nothing in them knows of the large rows."""
+import numpy as np
+import pytest
+
+from test_gpu_window_edges import _forward_backward, _inputs
+from window_reference import assert_within, attention
+
+pytestmark = pytest.mark.gpu
+
+SPREADS = [8, 16, 20, 30, 60]
+# (B, H, Hkv, L, window): in the first two four wavefronts have a workgroup's rows for themselves, in the last two eight share them;
+# every one is too large for the kernel that takes few rows
+SHAPES = [(14, 4, 2, 230, 32), (40, 2, 2, 210, 20), (9, 4, 2, 461, 200), (8, 8, 8, 500, 220)]
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from dl4s_amd import lib
+    c = lib.Context(0)
+    yield c
+    c.close()
+
+
+def _scale(d):
+    return float(np.float32(1 / np.sqrt(d)))
+
+
+def _ends(*tensors):
+    """The first and the last batch element, which are compared."""
+    return [x[[0, -1]] for x in tensors]
+
+
+def _compare(got, want, names, rows, what):
+    for name in names:
+        value, bound = (x[:, :, rows] for x in want[name])
+        assert_within(got[name][[0, -1]][:, :, rows], (value, bound), "%s of %s" % (name, what))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("r", SPREADS)
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+def test_rows_behind_larger_ones(ctx, which, r, d, shape):
+    """The first 64 rows of one tensor are of size one, the others of size 2^-r: results of what sees only the others.  Where that
+    would make the scores tiny, the other factor is 2^r times as large for the rows that meet only small ones."""
+    B, H, Hkv, L, window = shape
+    tensors = dict(zip(("q", "k", "v", "dout"), _inputs(np.random.default_rng(r + d), B, H, Hkv, L, L, d)))
+    tensors[which][:, :, 64:] *= np.float32(2.0 ** -r)
+    if which == "q":
+        tensors["k"][:, :, 64:] *= np.float32(2.0 ** r)     # seen by queries from 64 on
+    if which == "k":
+        tensors["q"][:, :, 64 + window:] *= np.float32(2.0 ** r)        # see keys from 65 on
+    got = _forward_backward(ctx, *tensors.values(), _scale(d), window)
+    tensors[which][:, :, :64] = 0
+    q, k, v, g = _ends(*tensors.values())
+    want = attention(q, k, v, _scale(d), window, dout=g)
+    # rows from 64 + window on neither see the first 64 nor are seen by them
+    _compare(got, want, ("dq", "dk", "dv") + (("out",) if which != "v" else ()), slice(64 + window, L), "rows behind larger " + which)
