@@ -327,7 +327,10 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_f32(const float *x, co
     const float ge = dentropy ? dentropy[row] : 0.f, H = ge == 0.f ? 0.f : stats[3 * row + 2];
     const float *xr = x + row * stride;
     float *dr = dx + row * stride;
+    // A row that no gradient reaches gets zeros, whatever stands in it (padding: an ignored target, tokens that are all blocked).
+    const bool none = gl == 0.f && ge == 0.f;
     auto gradient = [&](const float v, const long long j) {
+        if (none) return 0.f;
         float y = scaled(v, t) - m;
         y = y < -1e4f ? -1e4f : y;                                     // (a NaN stays)
         // (not from log p: the subtraction of L rounds by as much as a far z)

@@ -508,7 +508,8 @@ int dl4s_hip_token_logprobs_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t 
                                 float *stats, int64_t top_k, float *top_logprobs, int32_t *top_tokens);
 /* dlogits [rows, n] (rows row_stride apart; may be logits itself; columns from n on are left as they are) for the upstream
  * gradients dlogprobs [rows] and dentropy [rows], each of which may be NULL.  An ignored row takes no gradient through its
- * log probability, a target outside [0, n) gives NaN. */
+ * log probability, a target outside [0, n) gives NaN.  A row whose upstream gradients are zero or ignored gets zeros, whatever its
+ * logits are. */
 int dl4s_hip_token_logprobs_bwd_f32(dl4s_hip_ctx *ctx, const float *logits, int64_t rows, int64_t n, int64_t row_stride,
                                     float inv_temperature, const int32_t *targets, int32_t ignore_index, const float *stats,
                                     const float *dlogprobs, const float *dentropy, float *dlogits);

@@ -100,3 +100,28 @@ def test_logits_from_end_to_end_of_the_range(ctx, n):
     x[3] = np.where(np.arange(n) % 2, LOWEST, 0.0)
     for top in (0, 7):
         _check(ctx, x, n, targets=np.array([n - 1, 0, n // 2, 2]), top=top, grads=True, what="range")
+
+
+@pytest.mark.parametrize("n", [1, 63, 1000, 5001, 9000])
+def test_ignored_rows_of_blocked_tokens(ctx, n):
+    """Padding: every logit -inf, or NaN, the target ignored.  Nothing flows back into such a row, and its log probability is zero."""
+    rng = np.random.default_rng(n)
+    rows = 6
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    targets, g, h = rng.integers(0, n, rows), rng.standard_normal(rows).astype(np.float32), np.zeros(rows, np.float32)
+    x[1], x[3], x[4] = -np.inf, np.nan, np.inf
+    targets[[1, 3, 4, 5]] = -1
+    d, bound = _gradient_of_log_probabilities(x[[0, 2]], 0.9, targets[[0, 2]], g[[0, 2]])
+    for up in (None, h):
+        got = _gradient(ctx, x, 0.9, targets, -1, g, h=up)
+        assert not got[[1, 3, 4, 5]].any(), "padding rows"
+        _close(got[[0, 2]], d, bound, "rows between padding")
+
+
+def test_rows_that_no_gradient_reaches(ctx):
+    """An upstream gradient of zero is no gradient, in rows with targets too; a target outside the vocabulary stays NaN."""
+    x = np.random.default_rng(2).standard_normal((4, 300)).astype(np.float32)
+    x[0], x[3] = -np.inf, -np.inf
+    targets = np.array([5, 5, 300, 7])
+    got = _gradient(ctx, x, 1.0, targets, -1, np.array([0, 0, 0, 1.0], np.float32))
+    assert not got[:2].any() and np.isnan(got[2]).all() and np.isnan(got[3]).all()
