@@ -3,9 +3,10 @@
 // A value x is held as two fp16 planes of x times a power of two, x 2^a = h + l with h = fp16(x 2^a), l = fp16(x 2^a - h),
 // each rounded to nearest: 11 + 11 significant bits.  A product is three matrix instructions, l.h + h.l + h.h (the small ones
 // first), summed in fp32; the one left out is below 2^-22 of the product.  The power of two is shared: by a row for an operand
-// in registers, whose largest finite value it puts at 2^14 or more, and by what a wavefront has staged so far for one in
-// LDS (2^11 or more).  Nothing overflows, and what a value loses is 2^-23 of it or, where that is more, 2^-39 (2^-36) of
-// that largest: a tensor whose rows differ by up to 2^13 in size is as exact as in fp32 row by row.  Measured
+// in registers, whose largest finite value it puts at 2^14 or more, and by the 8, 16 or 32 neighbouring rows (above 64, above 32, up to 32
+// columns) that a wavefront stages at a time for one in LDS: 2^11 or more, or 2^7 where rows up to 2^8 times as large were staged
+// before.  Nothing overflows, and what a value loses is 2^-23 of it or, where that is more, 2^-39 (2^-36, 2^-32) of that
+// largest: neighbouring rows that differ by up to 2^13 (2^9) in size are as exact as in fp32 row by row.  Measured
 // against 64 bits, sums of 64 (512) products of normal values are off by 1.2e-7 (2.5e-7) of their size this way, 1.5e-7
 // (3.8e-7) through v_mfma_f32_32x32x2_f32.  Why: a 32 x 32 x 16 step costs 3 x 39 SIMD cycles (measured) where eight fp32
 // steps cost 8 x 66, and the vector ALU runs beside the fp16 instructions, not beside the fp32 ones.  Three bf16 planes
@@ -313,7 +314,18 @@ struct Stage {
     f32x4 x[NP][4];
     unsigned from[NP];       // byte offset of the thread's piece in its tensor's tile
     int to_row[NP], to_col[NP];
-    int run[2] = {MOST_POWER, MOST_POWER};   // smallest power so far of the rows this wavefront stages of either tile
+    // The power of the rows that this wavefront staged last of either tile, as the bits of the least number that keeps it: numbers from
+    // there up to 2^8 times as much do.
+    unsigned kept[2] = {least_of(MOST_POWER), least_of(MOST_POWER)};
+    __device__ static __forceinline__ constexpr unsigned least_of(const int a) { return (unsigned)(134 - a) << 23; }
+    __device__ static __forceinline__ int power_of(const unsigned least) { return 134 - (int)(least >> 23); }
+    // The power of rows whose largest value is m, and scaled m, behind rows with the power `last`.  Rows of zeros, and rows that would
+    // take a power one step (2^4) above the last one, take the last one: sizes that lie about a step's border then keep one
+    // power.  Smaller rows get their own, so that no row is rounded to the size of one that was staged long before it.
+    __device__ static __forceinline__ int next_power(const int last, const float m, const float scaled) {
+        const int own = coarse_scale_of(scaled);
+        return own <= last + 4 || m == 0.f ? min(last, own) : own;
+    }
 
     const int tid, wave0;    // the thread's number, and its wavefront's first, in the order in which wavefronts are given pieces
 
@@ -365,11 +377,14 @@ struct Stage {
         for (int i = 0; i < NP; ++i) {
             if (!has(i)) continue;
             const bool b = second(i);
-            float m = wave_max_abs(largest(x[i]));
-            if (__builtin_expect(m == INFINITY, 0)) m = wave_max_abs(largest_finite(x[i]));
             const float f = b ? 1.0f : fa;
-            int &least = QUADS % NT == 0 ? run[b] : run[0];       // (a wavefront has either pieces of one tile only, or these in turn)
-            const int a = least = min(least, coarse_scale_of(m * fabsf(f))), lane = threadIdx.x & 63;
+            unsigned &keeps = QUADS % NT == 0 ? kept[b] : kept[0];       // (a wavefront has either pieces of one tile only, or these in turn)
+            float m = wave_max_abs(largest(x[i]));
+            if (__builtin_expect(__builtin_amdgcn_readfirstlane(__float_as_uint(m * fabsf(f))) - keeps >= 8u << 23, 0)) {
+                if (m == INFINITY) m = wave_max_abs(largest_finite(x[i]));
+                keeps = least_of(next_power(power_of(keeps), m, m * fabsf(f)));
+            }
+            const int a = power_of(keeps), lane = threadIdx.x & 63;
             if (lane < WAVE_ROWS / 8) powers[(b ? R / 8 : 0) + ((wave0 + NT * i - b * QUADS) / GROUPS >> 1) + lane] = -a;
             if (b) put<ROWS_B, COLS_B>(i, rows_b, cols_b, pow2(a));
             else put<ROWS_A, COLS_A>(i, rows_a, cols_a, pow2(a) * f);
