@@ -437,6 +437,18 @@ __device__ __forceinline__ float to_one_unit(const Powers &p, int &n, f32x16 &op
     return pow2(max(was - n, -200));
 }
 
+// The same in units that follow the tile's powers down as well, so that a column that met none of the large rows does not have its
+// operand taken down: n is the tile's largest one, or 2^-60 of the largest so far.  What has been summed is then at most 2^120
+// units (operands and planes of up to 2^15, 2^30 rows, 2^60 of a step down), which fp32 holds.
+__device__ __forceinline__ float to_unit_of_tile(const Powers &p, int &n, int &most, f32x16 &operand) {
+    const int was = n;
+    most = max(most, p.hi);
+    n = max(p.hi, most - 60);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) operand[r] *= __builtin_ldexpf(1.0f, p.n[r >> 2] - n);
+    return pow2(max(was - n, -200));
+}
+
 // Row of register r of a 32 x 32 accumulator in the lane's half of the wavefront (the column is lane % 32).
 __device__ __forceinline__ constexpr int acc_row(const int r) { return 8 * (r >> 2) + (r & 3); }
 

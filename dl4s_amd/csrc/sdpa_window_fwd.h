@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256 * KS, DT <= 64 && KS == 1 ? 3 : 2) void sdpa_wi
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
     float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
-    int nv = -MOST_POWER;                                          // o is in units of 2^nv
+    int nv = -MOST_POWER, nv_most = -MOST_POWER;          // o is in units of 2^nv; the largest of them so far
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256 * KS, DT <= 64 && KS == 1 ? 3 : 2) void sdpa_wi
                 l_run += s[r];
             }
             if (vs.lo != nv || vs.hi != nv) {
-                const float unit = to_one_unit(vs, nv, s);
+                const float unit = to_unit_of_tile(vs, nv, nv_most, s);
 #pragma unroll
                 for (int t = 0; t < DT / 32; ++t) o[t] *= unit;
             }

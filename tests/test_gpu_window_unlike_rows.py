@@ -43,7 +43,7 @@ def _compare(got, want, names, rows, what):
 @pytest.mark.parametrize("shape", SHAPES)
 @pytest.mark.parametrize("d", [32, 64, 96, 128])
 @pytest.mark.parametrize("r", SPREADS)
-@pytest.mark.parametrize("which", ["q", "k", "dout"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
 def test_rows_behind_larger_ones(ctx, which, r, d, shape):
     """The first 64 rows of one tensor are of size one, the others of size 2^-r: results of what sees only the others.  Where that
     would make the scores tiny, the other factor is 2^r times as large for the rows that meet only small ones."""
@@ -60,3 +60,42 @@ def test_rows_behind_larger_ones(ctx, which, r, d, shape):
     want = attention(q, k, v, _scale(d), window, dout=g)
     # rows from 64 + window on neither see the first 64 nor are seen by them
     _compare(got, want, ("dq", "dk", "dv") + (("out",) if which != "v" else ()), slice(64 + window, L), "rows behind larger " + which)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("r", SPREADS + [-30])
+def test_outputs_behind_larger_values(ctx, r, d, shape):
+    """Queries of one wavefront, some of which see values 2^r times as large as all the others'."""
+    B, H, Hkv, L, window = shape
+    q, k, v, g = _inputs(np.random.default_rng(r + d + 200), B, H, Hkv, L, L, d)
+    at = slice(32, 64)
+    v[:, :, at] *= np.float32(2.0 ** r)
+    got = _forward_backward(ctx, q, k, v, g, _scale(d), window)
+    v[:, :, at] = 0
+    want = attention(*_ends(q, k, v), _scale(d), window)
+    for rows in (slice(0, 32), slice(63 + window, L)):
+        _compare(got, want, ["out"], rows, "rows beside larger values")
+
+
+@pytest.mark.parametrize("sizes", [(2.0 ** 110, 2.0 ** -60, 1.0), (2.0 ** -110, 2.0 ** 100, 2.0 ** -90)])
+@pytest.mark.parametrize("shape", SHAPES[:3:2])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_of_all_sizes(ctx, d, shape, sizes):
+    """Neighbouring tiles at opposite ends of the range of fp32: no sum leaves it, and a row that sees only one of the sizes has that
+    size's precision within 2^-60 of the largest."""
+    B, H, Hkv, L, window = shape
+    window = 16
+    q, k, v, g = _inputs(np.random.default_rng(d), B, H, Hkv, L, L, d)
+    step = np.arange(L) // 64 % 3
+    v *= np.asarray(sizes, np.float32)[step][None, None, :, None]
+    out = _forward_backward(ctx, q, k, v, g, _scale(d), window)["out"]
+    assert np.isfinite(out).all()
+    for n, size in enumerate(sizes):
+        part = np.where((step == n)[None, None, :, None], v, 0)
+        value, bound = attention(*_ends(q, k, part), _scale(d), window)["out"]
+        rows = (step == n) & (np.arange(L) % 64 >= window) & (np.arange(L) >= window)
+        # beside the bound: each of the window's weights off by half a step of its low plane, 2^-25, times planes of up to 2^15, in units
+        # of 2^-60 of those that hold the largest value (below 8 sizes, and 2^11 units or more), over a sum of weights of 2^7 or more
+        beside = window * 2.0 ** (-25 + 15 - 60 - 11 - 7) * 8 * max(sizes)
+        assert_within(out[[0, -1]][:, :, rows], (value[:, :, rows], bound[:, :, rows] + beside), "size %g" % size)
