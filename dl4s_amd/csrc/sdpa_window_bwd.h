@@ -13,7 +13,7 @@
 //     last kernel adds up in order; so are all blocks where that shortens the longest queue of a compute unit.
 // The size of dS, and of the weights a key gets, is not known beforehand: as operands they carry a power of two per column
 // (query or key), set by the first tile so that the largest value there is 2^8 and lowered, with the accumulators, when a
-// later one would pass 2^15.
+// later one, weighed with the size of the rows it is multiplied with, would pass 2^15.
 // Seven products for the five of the gradient, each three matrix instructions per 16-deep step, and the vector instructions of
 // the splitting, which every tile goes through in both forms, rows and columns: their issue bounds both kernels (B2 H16/4 L4096
 // d96 window 777: dq 229 us with the matrix pipe 32 % busy, dk/dv 392 us, 23 %).
@@ -22,45 +22,54 @@
 
 namespace {
 
-// The power of two that an operand carries in a lane's column: the operand is x * factor, factor = base * 2^c.  fit and
-// fit_tiny look at a tile's x before they are multiplied, whose size is that of fp32 numbers, and return whether any lane's power
-// moved; acc_factor is then the lane's factor for what it has accumulated.
-struct ColumnScale {
+// The unit 2^u of the sums in a lane's column.  A tile's operand is x * factor, factor = base * 2^(hi - u), where 2^hi is the unit of
+// the planes that it is multiplied with.  fit and fit_tiny look at a tile's x before they are multiplied, whose size is that of
+// fp32 numbers, and return whether any lane's unit rose; acc_factor is then the lane's factor for what it has accumulated.  A unit
+// rises by what the column itself meets (x and the planes' size together): large rows that only other columns meet leave it alone.
+struct ColumnUnit {
     const float base;
     float factor;
-    int c = 0;
-    bool fresh = true;
-    __device__ __forceinline__ explicit ColumnScale(const float b) : base(b), factor(b) {}
+    int u = 0;
+    bool fresh = true;                                     // nothing but zeros so far
+    __device__ __forceinline__ explicit ColumnUnit(const float b) : base(b), factor(b) {}
 
-    // the largest, m, to 2^8
-    __device__ __forceinline__ void move(const bool moves, const float m, const int least, float &acc_factor) {
-        const int to = moves ? min(max(135 - (int)(__float_as_uint(m * base) >> 23), least), 126) : c;
-        acc_factor = pow2(to - c);
-        c = to;
-        factor = base * pow2(c);
+    __device__ __forceinline__ void move(const int to, const int hi, float &acc_factor) {
+        acc_factor = pow2(max(min(u - to, 0), -200));      // (fresh columns, which may go down, hold zeros)
+        u = to;
+        set(hi);
     }
-    __device__ __forceinline__ bool fit(const f32x16 &x, float &acc_factor) {
+    // (a column of zeros may be any number of steps from the tile's unit: 0 times a finite factor)
+    __device__ __forceinline__ void set(const int hi) { factor = fminf(__builtin_ldexpf(base, hi - u), 3.40282347e38f); }
+    // the unit that takes m to 2^8
+    __device__ __forceinline__ int unit_for(const float m, const int hi) const {
+        return hi - min(max(135 - (int)(__float_as_uint(m * base) >> 23), -126), 126);
+    }
+    __device__ __forceinline__ bool fit(const f32x16 &x, const int hi, float &acc_factor) {
         float m = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(x[r]));
-        if (!__any(m * factor > 32768.0f || (fresh && m > 0.f))) return false;
+        const float f = __builtin_ldexpf(base, hi - u);
+        factor = fminf(f, 3.40282347e38f);
+        if (!__any(m * f > 32768.0f || (fresh && m > 0.f))) return false;
         m = max_halves(m);
-        const bool moves = m * factor > 32768.0f || (fresh && m > 0.f);
+        const bool moves = m * f > 32768.0f || (fresh && m > 0.f);
         fresh = fresh && !(m > 0.f);
-        move(moves, m, -126, acc_factor);
+        move(moves ? unit_for(m, hi) : u, hi, acc_factor);
         return true;
     }
-    // For weights, which are at most 2^13: a column takes a power only where its first largest is below 2^-3.
-    __device__ __forceinline__ bool fit_tiny(const f32x16 &w, float &acc_factor) {
+    // For weights, which are at most 2^13: a column takes the tile's unit where its largest is 2^-3 or more.
+    __device__ __forceinline__ bool fit_tiny(const f32x16 &w, const int hi, float &acc_factor) {
         float m = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, w[r]);
         m = max_halves(m);
-        const bool moves = (c != 0 && m * factor > 32768.0f) || (fresh && m > 0.f && m < 0.125f);
+        int to = u;
+        if (m >= 0.125f) to = fresh ? hi : max(u, hi);
+        else if (m > 0.f && (fresh || __builtin_ldexpf(m, hi - u) > 32768.0f)) to = unit_for(m, hi);
+        const bool rises = !fresh && to > u;
         fresh = fresh && !(m > 0.f);
-        if (!__any(moves)) return false;
-        move(moves, m, 0, acc_factor);
-        return true;
+        move(to, hi, acc_factor);
+        return __any(rises);
     }
 };
 
@@ -76,9 +85,9 @@ __device__ __forceinline__ void window_dq(const float *__restrict__ q, const flo
     u16 *Ks = window_lds, *Vs = Ks + 2 * T::ROWS_PLANE, *Kc = Vs + 2 * T::ROWS_PLANE;
     __shared__ __align__(16) int powers[2][BN / 8];        // [K, V]
 
-    const int unit = (workgroup & 7) * g.per_xcd + (workgroup >> 3);
-    if (unit >= g.units) return;
-    const Place<BN> at(g, unit);
+    const int place = (workgroup & 7) * g.per_xcd + (workgroup >> 3);
+    if (place >= g.units) return;
+    const Place<BN> at(g, place);
     const int half = (threadIdx.x & 63) >> 5, part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
 
     const float *kp = k + at.b * g.lk.b + at.hk * g.lk.h, *vp = v + at.b * g.lk.b + at.hk * g.lk.h;
@@ -112,8 +121,7 @@ __device__ __forceinline__ void window_dq(const float *__restrict__ q, const flo
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-    ColumnScale scale(inv);                                // dS = 2^(s - m) (dP - delta) / l
-    int nk = -MOST_POWER;                                          // acc is in units of 2^nk
+    ColumnUnit unit(inv);                                  // dS = 2^(s - m) (dP - delta) / l
 
     for (int i = 0; i < at.tiles; ++i) {
         __syncthreads();
@@ -141,19 +149,15 @@ __device__ __forceinline__ void window_dq(const float *__restrict__ q, const flo
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = sees(g.w, p, k0 + acc_row(r) + 4 * half, at.len) ? s[r] : 0.f;
         }
-        if (kn.lo != nk || kn.hi != nk) {
-            const float unit = to_one_unit(kn, nk, s);
-#pragma unroll
-            for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
-        }
+        if (kn.lo != kn.hi) to_one_unit(kn, s);
         float shrink;
-        if (scale.fit(s, shrink)) {
+        if (unit.fit(s, kn.hi, shrink)) {
 #pragma unroll
             for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
         }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            const Frag df = acc_frag(s, st, scale.factor);
+            const Frag df = acc_frag(s, st, unit.factor);
             Frag kc[DT / 32];
 #pragma unroll
             for (int t = 0; t < DT / 32; ++t) kc[t] = T::cols_frag(Kc, t, 2 * part + st);
@@ -163,7 +167,7 @@ __device__ __forceinline__ void window_dq(const float *__restrict__ q, const flo
 
 #pragma unroll
     for (int t = 0; t < DT / 32; ++t) settle(acc[t]);
-    const int power = nk - scale.c;
+    const int power = unit.u;
     f32x4 *sums = reinterpret_cast<f32x4 *>(window_lds);                 // KS = 2: [wavefront][DT / 8][lane], over the tiles
     const int at_sums = ((threadIdx.x >> 6) & 3) * (DT / 8) * 64 + (threadIdx.x & 63);
     if (KS == 2) {
@@ -307,10 +311,10 @@ __device__ __forceinline__ void window_dkv(const float *__restrict__ q, const fl
     for (int t = 0; t < DT / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-    // The operands are 2^13 w, times a power of two where a column's weights are all tiny, and w (dP - delta) factor.
-    ColumnScale scale(values ? 1.0f / 8192 : 1.0f);
-    bool plain = false;                                    // every column has met a weight that needs no power
-    int unit_power = -MOST_POWER;                                  // acc is in units of 2^unit_power
+    // The operands are 2^13 w, and w (dP - delta).
+    ColumnUnit column(values ? 1.0f / 8192 : 1.0f);
+    bool plain = false;                                    // every column is in units of 2^plain_unit, and its weights need no factor there
+    int plain_unit = 0;
 
     // Two buffers: behind the exchange of the weights one wavefront of a pair multiplies and then stages its share of the next
     // tile, the other stages first, so that on their SIMD one's vector work runs beside the other's matrix instructions.
@@ -372,19 +376,16 @@ __device__ __forceinline__ void window_dkv(const float *__restrict__ q, const fl
                 }
             }
             const Powers pw(powers[buf][!values]);
-            if (pw.lo != unit_power || pw.hi != unit_power) {
-                const float unit = to_one_unit(pw, unit_power, s);
-#pragma unroll
-                for (int t = 0; t < DT / 32; ++t) acc[t] *= unit;
-            }
-            if (values || !plain) {
+            if (pw.lo != pw.hi) to_one_unit(pw, s);
+            if (values || !plain || pw.lo != plain_unit || pw.hi != plain_unit) {
                 float shrink;
-                if (values ? scale.fit(s, shrink) : scale.fit_tiny(s, shrink)) {
+                if (values ? column.fit(s, pw.hi, shrink) : column.fit_tiny(s, pw.hi, shrink)) {
 #pragma unroll
                     for (int t = 0; t < DT / 32; ++t) acc[t] *= shrink;
                 }
-                s *= scale.factor;
-                plain = !__any(scale.fresh || scale.c != 0);
+                s *= column.factor;
+                plain = !__any(column.fresh || column.u != pw.hi);
+                plain_unit = pw.hi;
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
@@ -403,7 +404,7 @@ __device__ __forceinline__ void window_dkv(const float *__restrict__ q, const fl
     for (int t = 0; t < DT / 32; ++t) settle(acc[t]);
     if (key >= g.Lk) return;
     // q was staged as q rT log2(e): dk = rT sum dS q = ln(2) of what was summed
-    const int power = unit_power - scale.c - (values ? 0 : 13);
+    const int power = column.u - (values ? 0 : 13);
     const float factor_out = values ? 0.69314718055994530942f : 1.0f;
     float *to_row = (values ? dk : dv) + el;
     if (kb.chunks[cl] > 1) to_row = partial_sums(kb, pair, block, chunk, g.d) + (values ? 0 : 128ll * g.d) + (two * 32 + ln) * (long long)g.d;

@@ -427,19 +427,15 @@ struct Powers {
         hi = __builtin_amdgcn_readfirstlane(max(max(n.x, n.y), max(n.z, n.w)));
     }
 };
-// What is summed over rows with powers of their own is kept in units of 2^n, n the largest so far.  An operand's registers r
-// that stand for a row with a smaller one are taken down to it; returns the factor for what has been summed before.
-__device__ __forceinline__ float to_one_unit(const Powers &p, int &n, f32x16 &operand) {
-    const int was = n;
-    n = max(n, p.hi);
+// The operand's registers r stand for rows with powers of their own: those that stand for smaller ones are taken down to 2^hi.
+__device__ __forceinline__ void to_one_unit(const Powers &p, f32x16 &operand) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) operand[r] *= __builtin_ldexpf(1.0f, p.n[r >> 2] - n);
-    return pow2(max(was - n, -200));
+    for (int r = 0; r < 16; ++r) operand[r] *= __builtin_ldexpf(1.0f, p.n[r >> 2] - p.hi);
 }
-
-// The same in units that follow the tile's powers down as well, so that a column that met none of the large rows does not have its
-// operand taken down: n is the tile's largest one, or 2^-60 of the largest so far.  What has been summed is then at most 2^120
-// units (operands and planes of up to 2^15, 2^30 rows, 2^60 of a step down), which fp32 holds.
+// The same for sums that are kept in units of 2^n for all columns alike; returns the factor for what has been summed before.  n
+// follows the tiles down as well, so that a column that met none of the large rows does not have its operand taken down: it is
+// the tile's 2^hi, or 2^-60 of the largest so far.  What has been summed is then at most 2^120 units (operands and planes of up
+// to 2^15, 2^30 rows, 2^60 of a step down), which fp32 holds.
 __device__ __forceinline__ float to_unit_of_tile(const Powers &p, int &n, int &most, f32x16 &operand) {
     const int was = n;
     most = max(most, p.hi);

@@ -99,3 +99,41 @@ def test_values_of_all_sizes(ctx, d, shape, sizes):
         # of 2^-60 of those that hold the largest value (below 8 sizes, and 2^11 units or more), over a sum of weights of 2^7 or more
         beside = window * 2.0 ** (-25 + 15 - 60 - 11 - 7) * 8 * max(sizes)
         assert_within(out[[0, -1]][:, :, rows], (value[:, :, rows], bound[:, :, rows] + beside), "size %g" % size)
+
+
+@pytest.mark.parametrize("r", SPREADS)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("B,H,Hkv,L,window", [(2, 4, 1, 200, 8), (20, 8, 4, 200, 8), (3, 6, 2, 300, 8)])
+def test_shared_heads_beside_larger_rows(ctx, r, d, B, H, Hkv, L, window):
+    """Query heads of a group, one after the other: rows that some keys of a wavefront see are larger in every head, and the sums
+    of the keys that do not see them go on in the next head as exactly as they began."""
+    at = slice(32, 64)
+    for which in (0, 3):                                    # q: dk; dout: dk and dv
+        tensors = _inputs(np.random.default_rng(r + d + 300), B, H, Hkv, L, L, d)
+        large = tensors[which][:, :, at].copy()
+        tensors[which] *= np.float32(2.0 ** -r)
+        tensors[which][:, :, at] = large
+        got = _forward_backward(ctx, *tensors, _scale(d), window)
+        tensors[which][:, :, at] = 0
+        q, k, v, g = _ends(*tensors)
+        want = attention(q, k, v, _scale(d), window, dout=g)
+        for keys in (slice(0, 25), slice(64, L)):           # key 24 is seen up to row 31, key 64 from row 64 on
+            _compare(got, want, ("dk", "dv"), keys, "shared heads")
+
+
+@pytest.mark.parametrize("r", SPREADS)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("B,H,Hkv,L,window", [(2, 2, 2, 300, 70), (24, 4, 2, 300, 70), (12, 2, 2, 600, 230)])
+def test_query_gradients_beside_larger_keys(ctx, r, d, B, H, Hkv, L, window):
+    """Queries that see the first keys and their window, between them keys that only other queries of the same wavefront see: these
+    are 2^r times as large, and the queries 2^-r times, so that all scores are ordinary ones."""
+    sinks, at = 4, slice(96, 128)
+    q, k, v, g = _inputs(np.random.default_rng(r + d + 400), B, H, Hkv, L, L, d)
+    q *= np.float32(2.0 ** -r)
+    k[:, :, at] *= np.float32(2.0 ** r)
+    got = _forward_backward(ctx, q, k, v, g, _scale(d), window, sinks)
+    k[:, :, at] = 0
+    q, k, v, g = _ends(q, k, v, g)
+    want = attention(q, k, v, _scale(d), window, sinks, dout=g)
+    for rows in (slice(0, 96), slice(127 + window, L)):
+        _compare(got, want, ["dq"], rows, "queries beside larger keys")
