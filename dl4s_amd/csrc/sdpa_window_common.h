@@ -147,8 +147,8 @@ struct Planes {
     unsigned h, l;
 };
 // v_fma_mixlo_f16 / v_fma_mixhi_f16 round an fp32 multiply-add to fp16 into the low / high half of their result.  A half that was
-// moved up may be read one wait state later at the earliest; the compiler does not look into the statement, so it ends
-// with that state.
+// moved up may be read one wait state later at the earliest, and a matrix instruction reads what a vector instruction wrote
+// two wait states later; the compiler does not look into the statement, so it ends with these two.
 __device__ __forceinline__ unsigned round2(const float a, const float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
@@ -162,7 +162,7 @@ __device__ __forceinline__ void split4(const f32x4 v, const float s, Planes &p, 
         "v_fma_mixhi_f16 %1, %5, %8, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
         "v_fma_mixlo_f16 %3, %6, %8, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
         "v_fma_mixhi_f16 %3, %7, %8, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
-        "s_nop 0"
+        "s_nop 1"
         : "=&v"(p.h), "=&v"(p.l), "=&v"(q.h), "=&v"(q.l)
         : "v"(v.x), "v"(v.y), "v"(v.z), "v"(v.w), "v"(s));
 }
@@ -184,7 +184,7 @@ __device__ __forceinline__ Frag split8(const float (&x)[8]) {
         "v_fma_mixhi_f16 %1, %7, 1.0, -%13 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
         "v_fma_mixhi_f16 %2, %9, 1.0, -%14 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
         "v_fma_mixhi_f16 %3, %11, 1.0, -%15 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
-        "s_nop 0"
+        "s_nop 1"
         : "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3)
         : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]), "v"(h.x), "v"(h.y), "v"(h.z), "v"(h.w));
     l = u32x4{l0, l1, l2, l3};
