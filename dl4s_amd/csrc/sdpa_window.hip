@@ -212,7 +212,8 @@ int launch_fwd_width(dl4s_hip_ctx *ctx, const float *q, const float *k, const fl
 // second launch that adds up partial sums about three, and their way through memory); those with first keys, which
 // every later query sees, into enough pieces to give every compute unit one.  At most 2048 workgroups leave partial sums.
 // beside: the workgroups share the GPU with those of dq; they are to be no more than the compute units that those leave.
-KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B, bool beside) {
+// *partial_bytes: what the partial sums take (1 KiB of d for each workgroup that leaves some); kb.partial is set by the caller.
+KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B, bool beside, size_t *partial_bytes) {
     KeyBlocks kb;
     kb.pairs = (int)(B * g.Hkv);
     kb.blocks = (g.Lk + 127) / 128;
@@ -239,7 +240,8 @@ KeyBlocks key_blocks(const dl4s_hip_ctx *ctx, const WindowGeometry &g, int64_t B
     }
     const long long floats0 = kb.chunks[0] > 1 ? kb.units[0] * 256ll * g.d : 0, floats1 = kb.chunks[1] > 1 ? kb.units[1] * 256ll * g.d : 0;
     kb.class1 = floats0;
-    kb.partial = reinterpret_cast<float *>((floats0 + floats1) * sizeof(float));      // the caller replaces the size by the address
+    kb.partial = nullptr;
+    *partial_bytes = (size_t)(floats0 + floats1) * sizeof(float);
     return kb;
 }
 
@@ -442,14 +444,15 @@ int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
         // and 94, L64 21 and 13; d 96: 67 and 42, 153 and 117, 26 and 16; with two workgroups to a compute unit, B4 H8 L1024
         // window 128, 53 and 57); above 96 columns dq needs a SIMD's registers alone
         bool beside = d <= 96 && rows && krows && 2 * g.units <= ctx->cu_count;
-        KeyBlocks kb = krows ? key_blocks(ctx, g, B, beside) : KeyBlocks{};
+        size_t partial_bytes = 0;
+        KeyBlocks kb = krows ? key_blocks(ctx, g, B, beside, &partial_bytes) : KeyBlocks{};
         if (beside && g.units + kb.units[0] + kb.units[1] > ctx->cu_count) {
             beside = false;
-            kb = key_blocks(ctx, g, B, false);
+            kb = key_blocks(ctx, g, B, false, &partial_bytes);
         }
         rc = fits_a_launch("sdpa_window_bwd", std::max(8ll * g.per_xcd, 16ll * (kb.per_xcd[0] + kb.per_xcd[1])), 256);
         if (rc) return rc;
-        rc = dl4s::ensure_scratch(ctx, delta_bytes + reinterpret_cast<size_t>(kb.partial));
+        rc = dl4s::ensure_scratch(ctx, delta_bytes + partial_bytes);
         if (rc) return rc;
         float *delta = reinterpret_cast<float *>(ctx->scratch);
         kb.partial = delta + delta_bytes / sizeof(float);
