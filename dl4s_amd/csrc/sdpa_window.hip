@@ -375,8 +375,8 @@ int window_checks(const char *what, int64_t B, int64_t H, int64_t Hkv, int64_t L
                  (long long)H, (long long)Hkv);
     DL4S_REQUIRE(d >= 1 && d <= MAXD, DL4S_HIP_EUNSUPPORTED, "%s: head dim %lld (1 to %d are implemented)", what, (long long)d, MAXD);
     const int64_t big = int64_t(1) << 30, most = big - 256;
-    DL4S_REQUIRE(Lq <= most && Lk <= most && B < big && H < big && B * H < big && desc->q_offset <= most - Lq, DL4S_HIP_EUNSUPPORTED,
-                 "%s: more than 2^30 heads, or a position above 2^30 - 256", what);
+    DL4S_REQUIRE(Lq <= most && Lk <= most && B < big && H < big && Hkv < big && B * H < big && B * Hkv < big && desc->q_offset <= most - Lq,
+                 DL4S_HIP_EUNSUPPORTED, "%s: more than 2^30 heads, or a position above 2^30 - 256", what);
     DL4S_REQUIRE(H * d <= (int64_t(1) << 22), DL4S_HIP_EUNSUPPORTED, "%s: %lld heads of %lld: a token's heads above 2^22 values", what,
                  (long long)H, (long long)d);
     DL4S_REQUIRE(B * H * Lq < big * 4 && B * Hkv * Lk < big * 4, DL4S_HIP_EUNSUPPORTED, "%s: more than 2^32 rows", what);
