@@ -7,7 +7,7 @@
 //     group.  Two wavefronts share 32 keys (the columns of their accumulators): one holds K and forms S = Q . K^T, the weights
 //     w, and dV^T += dO^T . w, the other holds V and forms dP = dO . V^T and, with the weights it gets through LDS,
 //     dK^T += Q^T . dS.  That halves what a wavefront keeps in registers, so two run on a SIMD at every head dim (one
-//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes 392 us at B2 H16/4 L4096 d96 window 777).
+//     wavefront for both, alone on its SIMD above 64 columns, took 655 us where this takes 395 us at B2 H16/4 L4096 d96 window 777).
 //     Shared key heads are summed in the accumulators, in a fixed order, without atomics.  Key blocks that hold visible
 //     first keys are seen by every later query: their query tiles are dealt to several workgroups whose partial sums a
 //     last kernel adds up in order; so are all blocks where that shortens the longest queue of a compute unit.
@@ -16,7 +16,7 @@
 // later one, weighed with the size of the rows it is multiplied with, would pass 2^15.
 // Seven products for the five of the gradient, each three matrix instructions per 16-deep step, and the vector instructions of
 // the splitting, which every tile goes through in both forms, rows and columns: their issue bounds both kernels (B2 H16/4 L4096
-// d96 window 777: dq 229 us with the matrix pipe 32 % busy, dk/dv 392 us, 23 %).
+// d96 window 777: dq 230 us with the matrix pipe 31 % busy, dk/dv 395 us, 23 %).
 #pragma once
 #include "sdpa_window_fwd.h"
 

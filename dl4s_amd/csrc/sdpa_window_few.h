@@ -66,7 +66,7 @@ __global__ __launch_bounds__(NW * 64, DT <= 64 ? 3 : (DT <= 128 ? 2 : 1)) void s
         for (int e = 0; e < 4; ++e) o[j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
 
-    // a row's four floats, once: nothing here is read again
+    // a row's four floats: this workgroup does not read them again (others of the same key head do, if it has more than 16 query rows)
     auto stream4 = [&](const float *row, const int c) -> f32x4 {
         if (!a.vec) return load4(row, c, a.d, false);
         return c < a.d ? __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(row + c)) : f32x4{0.f, 0.f, 0.f, 0.f};

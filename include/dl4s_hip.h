@@ -301,14 +301,23 @@ int dl4s_hip_argmax_to_f32(dl4s_hip_ctx *ctx, const float *values, int64_t count
  * What stands in masked places: rows at or beyond lengths[b], keys behind the last query's position and keys that lie before
  * the first query's window (and are none of the first) may hold anything, as may q and dout in rows that see no key.  A key
  * that some queries see and others do not has to be finite: its weight in the other rows is zero, and zero times NaN or
- * infinity is NaN there too.  An infinity among the operands of a visible pair gives NaN.
- * Precision: fp32 throughout; up to 128 columns the products are formed from two fp16 halves of each operand that share a
- * power of two along a row, or among the rows of k, v, q, dout that are read together, so a value also carries an error of up
- * to 2^-36 of the largest of those rows, a weight one of up to 2^-32 (sums of 64 products of like-sized values are off by 1.2e-7 of
- * their size, 1.5e-7 on the fp32 instructions).
- * Limits (DL4S_HIP_EUNSUPPORTED): H * d up to 2^22, q_offset + Lq and Lk up to 2^30 - 256, B * H below 2^30, fewer than 2^32 rows,
- * and 2^24 workgroups of a launch (of 128 rows, above 128 columns of 4; half as many of 16 for few rows).  The first call of a
- * shape may need the library's scratch block to grow, which a recording refuses: run the same call once before. */
+ * infinity is NaN there too.  What comes of an infinity among the operands of a visible pair depends on the kernel that the
+ * extents choose: NaN, or what fp32 arithmetic gives.
+ * Precision: fp32 throughout for few query rows and above 128 columns.  The other calls keep sums, scores and statistics in
+ * fp32 and form the products from two fp16 halves of each operand (22 bits) times a power of two, one for a row or for 8, 16 or 32
+ * neighbouring rows of a head (above 64, above 32, up to 32 columns).  Beside 2^-23 of itself a value of q, k, v, dout is off by up
+ * to 2^-36 of the largest among those rows (2^-32 where rows up to 2^8 times as large were read before), a weight by up to
+ * 2^-32 of its row's sum or 2^-33 of the largest that its key has, and a score's gradient by 2^-33 of the largest in its row (dq)
+ * or column (dk), each weighed with the largest of the 32 neighbouring rows that it is multiplied with (2^-25 where those differ
+ * in size from block to block).  Rows further away do not matter, whatever their size: neighbouring rows that differ by less
+ * than 2^9 are as exact as in fp32, a row that is 2^-20 of its neighbour has 12 to 16 bits.  (Sums of 64 products of like-sized
+ * values are off by 1.2e-7 of their size, 1.5e-7 on the fp32 instructions.)
+ * Limits (DL4S_HIP_EUNSUPPORTED): H * d up to 2^22, q_offset + Lq and Lk up to 2^30 - 256, B * H and B * Hkv below 2^30, fewer than
+ * 2^32 rows, and 2^24 workgroups of a launch (of 128 rows, above 128 columns of 4; half as many of 16 for few rows).
+ * Scratch: the library's block; keys that several workgroups share take up to 512 * 16 * (d + 2) floats (8 MiB at 256 columns), the
+ * gradient call a float for every query row and, up to 128 columns where key blocks are dealt to several workgroups, up to d * 2560
+ * KiB of partial sums (320 MiB at 128 columns).  The first call of a shape may need the block to grow, which a recording
+ * refuses: run the same call once before. */
 typedef struct dl4s_window_desc {
     int64_t window;         /* >= 1: the query's own position and the window - 1 before it */
     int64_t sinks;          /* >= 0: the first keys, which stay visible to every later position */
@@ -322,7 +331,8 @@ int dl4s_hip_sdpa_window_fwd_f32(dl4s_hip_ctx *ctx, const float *q, const float 
                                  const dl4s_window_desc *window, uint32_t flags);
 /* dq, dk, dv for the upstream gradient dout, from the tensors of the forward call with the same extents, window and flags.
  * dk and dv are summed over the query heads that share a key head.  Deterministic: no atomics, the same bits on every run.
- * Uses the library's scratch block.  Above 128 columns simple kernels without matrix instructions form it. */
+ * Above 128 columns simple kernels without matrix instructions form it (B1 H16 L2048 d256 window 512, with the forward pass:
+ * 43 ms). */
 int dl4s_hip_sdpa_window_bwd_f32(dl4s_hip_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
                                  const float *stats, const float *dout, float *dq, float *dk, float *dv, int64_t B, int64_t H,
                                  int64_t Hkv, int64_t Lq, int64_t Lk, int64_t d, float inv_temperature, const dl4s_window_desc *window,
@@ -361,7 +371,8 @@ int dl4s_hip_rotary_frequencies(int64_t rot_dim, double base, int scaling, doubl
                                 int64_t original_length, double *out_turns);
 /* Queries and keys in one launch (either pair of pointers may be NULL with its head count 0); an output may be its input, and
  * may not overlap it otherwise.  positions: device int32 [B,L], or NULL for position0 + l; negative ones turn backwards.  d up to
- * 4096, B * L below 2^30, (H + Hkv) * d below 2^29. */
+ * 4096, B * L below 2^30, (H + Hkv) * d below 2^29, and below 2^24 workgroups of 8192 columns, or of one token where it has more (B * L
+ * below 2^24 from (H + Hkv) * d = 4097 on). */
 int dl4s_hip_rotary_f32(dl4s_hip_ctx *ctx, const float *q, float *q_out, const float *k, float *k_out, int64_t B, int64_t L, int64_t H,
                         int64_t Hkv, int64_t d, int64_t rot_dim, const double *turns, const int32_t *positions, int64_t position0,
                         float amplitude, uint32_t flags);
