@@ -319,12 +319,12 @@ struct Stage {
     unsigned kept[2] = {least_of(MOST_POWER), least_of(MOST_POWER)};
     __device__ static __forceinline__ constexpr unsigned least_of(const int a) { return (unsigned)(134 - a) << 23; }
     __device__ static __forceinline__ int power_of(const unsigned least) { return 134 - (int)(least >> 23); }
-    // The power of rows whose largest value is m, and scaled m, behind rows with the power `last`.  Rows of zeros, and rows that would
-    // take a power one step (2^4) above the last one, take the last one: sizes that lie about a step's border then keep one
-    // power.  Smaller rows get their own, so that no row is rounded to the size of one that was staged long before it.
-    __device__ static __forceinline__ int next_power(const int last, const float m, const float scaled) {
-        const int own = coarse_scale_of(scaled);
-        return own <= last + 4 || m == 0.f ? min(last, own) : own;
+    // The power of rows whose largest value is m behind rows with the power `last`.  Rows that would take a power one step (2^4) above
+    // the last one take the last one: sizes that lie about a step's border then keep one power.  Smaller rows get their own, so
+    // that no row is rounded to the size of one that was staged long before it.
+    __device__ static __forceinline__ int next_power(const int last, const float m) {
+        const int own = coarse_scale_of(m);
+        return own <= last + 4 ? min(last, own) : own;
     }
 
     const int tid, wave0;    // the thread's number, and its wavefront's first, in the order in which wavefronts are given pieces
@@ -380,11 +380,14 @@ struct Stage {
             const float f = b ? 1.0f : fa;
             unsigned &keeps = QUADS % NT == 0 ? kept[b] : kept[0];       // (a wavefront has either pieces of one tile only, or these in turn)
             float m = wave_max_abs(largest(x[i]));
+            int a = power_of(keeps);
             if (__builtin_expect(__builtin_amdgcn_readfirstlane(__float_as_uint(m * fabsf(f))) - keeps >= 8u << 23, 0)) {
                 if (m == INFINITY) m = wave_max_abs(largest_finite(x[i]));
-                keeps = least_of(next_power(power_of(keeps), m, m * fabsf(f)));
+                // (rows of zeros, a tile's missing ones among them, have no size that their neighbours would be weighed with)
+                if (m * fabsf(f) == 0.f) a = MOST_POWER;
+                else keeps = least_of(a = next_power(a, m * fabsf(f)));
             }
-            const int a = power_of(keeps), lane = threadIdx.x & 63;
+            const int lane = threadIdx.x & 63;
             if (lane < WAVE_ROWS / 8) powers[(b ? R / 8 : 0) + ((wave0 + NT * i - b * QUADS) / GROUPS >> 1) + lane] = -a;
             if (b) put<ROWS_B, COLS_B>(i, rows_b, cols_b, pow2(a));
             else put<ROWS_A, COLS_A>(i, rows_a, cols_a, pow2(a) * f);

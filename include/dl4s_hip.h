@@ -309,9 +309,9 @@ int dl4s_hip_argmax_to_f32(dl4s_hip_ctx *ctx, const float *values, int64_t count
  * to 2^-36 of the largest among those rows (2^-32 where rows up to 2^8 times as large were read before), a weight by up to
  * 2^-32 of its row's sum or 2^-33 of the largest that its key has, and a score's gradient by 2^-33 of the largest in its row (dq)
  * or column (dk), each weighed with the largest of the 32 neighbouring rows that it is multiplied with (2^-25 where those differ
- * in size from block to block).  Rows further away do not matter, whatever their size: neighbouring rows that differ by less
- * than 2^9 are as exact as in fp32, a row that is 2^-20 of its neighbour has 12 to 16 bits.  (Sums of 64 products of like-sized
- * values are off by 1.2e-7 of their size, 1.5e-7 on the fp32 instructions.)
+ * in size from block to block).  Rows further away do not matter, unless values of another query are more than 2^60 times as
+ * large: neighbouring rows that differ by less than 2^9 are as exact as in fp32, a row that is 2^-20 of its neighbour has 12 to
+ * 16 bits.  (Sums of 64 products of like-sized values are off by 1.2e-7 of their size, 1.5e-7 on the fp32 instructions.)
  * Limits (DL4S_HIP_EUNSUPPORTED): H * d up to 2^22, q_offset + Lq and Lk up to 2^30 - 256, B * H and B * Hkv below 2^30, fewer than
  * 2^32 rows, and 2^24 workgroups of a launch (of 128 rows, above 128 columns of 4; half as many of 16 for few rows).
  * Scratch: the library's block; keys that several workgroups share take up to 512 * 16 * (d + 2) floats (8 MiB at 256 columns), the

@@ -137,3 +137,20 @@ def test_query_gradients_beside_larger_keys(ctx, r, d, B, H, Hkv, L, window):
     want = attention(q, k, v, _scale(d), window, sinks, dout=g)
     for rows in (slice(0, 96), slice(127 + window, L)):
         _compare(got, want, ["dq"], rows, "queries beside larger keys")
+
+
+@pytest.mark.parametrize("r", SPREADS)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("B,H,Hkv,L,window,length", [(40, 2, 2, 230, 4, 230), (40, 2, 2, 230, 4, 198), (14, 4, 1, 197, 3, 197), (9, 4, 2, 461, 10, 461)])
+def test_last_rows_behind_larger_values(ctx, r, d, B, H, Hkv, L, window, length):
+    """A tile that ends with fewer than 32 keys, 2^-r times as large as those of the tiles before it: its missing rows have no size."""
+    q, k, v, g = _inputs(np.random.default_rng(r + d + 500), B, H, Hkv, L, L, d)
+    last = length // 32 * 32
+    v[:, :, last:] *= np.float32(2.0 ** -r)
+    got = _forward_backward(ctx, q, k, v, g, _scale(d), window, lengths=[length] * B)
+    v[:, :, :last] = 0
+    q, k, v, g = _ends(q, k, v, g)
+    want = attention(q, k, v, _scale(d), window, lengths=[length] * 2, dout=g)
+    _compare(got, want, ("out", "dq"), slice(last + window - 1, L), "the last rows")
+    # (a key's gradient takes in all queries that see it)
+    _compare(got, want, ("dk", "dv"), slice(last + window - 1, L), "the last rows")
